@@ -449,6 +449,74 @@ int stk_paged_append(const void* k_new, const void* v_new, int dtype, int reques
                      int32_t* nblocks, int32_t* ntokens, const int32_t* positions,
                      void* stream);
 
+/* New tokens of a ragged batch into the pool, any number per request, in one
+ * launch.  Request r's are rows [starts[r], starts[r + 1]) of k_new and v_new
+ * [tokens, Hkv, D] (k_stride, v_stride elements from one token to the next;
+ * heads and dims contiguous); the first of them goes to token position
+ * positions[r].  With cos and sin [rows, rot / 2] FP32 (rows >= nb * b) the
+ * keys are rotated to their positions: pairs (i, i + rot / 2) of the first
+ * rot dims, or (2i, 2i + 1) with interleaved != 0, in FP32, rounded once.  q
+ * [tokens, Hq, D] (may be null) is rotated likewise into q_out [tokens, Hq, D];
+ * its rows of no request, or at a position outside [0, rows), become zero.
+ * Every touched page's lo/hi take in the stored keys (a block whose first new
+ * token has offset 0 starts them over), nblocks[r] and ntokens[r] (when not
+ * null) become those of the request's end.  Tokens at positions outside [0, nb *
+ * b) and on invalid pages are not written; a request with any of them, or
+ * with no new token, keeps its counts.  starts must not decrease, a page that
+ * is written must belong to one request, and positions must not be the ntokens
+ * array.  FP16 / BF16, D in {64, 128, 256}, rot a multiple of 16, rows and
+ * pages 16-byte aligned, lo/hi as stk_paged_append. */
+int stk_paged_extend(const void* k_new, int64_t k_stride, const void* v_new, int64_t v_stride,
+                     const void* q, int64_t q_stride, void* q_out, int dtype, int tokens,
+                     int requests, int hq, int hkv, int nb, int b, int d, int pages,
+                     const int32_t* starts, const int32_t* positions, const float* cos,
+                     const float* sin, int rows, int rot, int interleaved, void* k_pages,
+                     void* v_pages, void* lo_pages, void* hi_pages, int bounds_dtype,
+                     const int32_t* block_table, int32_t* nblocks, int32_t* ntokens,
+                     void* stream);
+
+size_t stk_paged_attention_workspace_bytes(int tokens, int requests, int hq, int hkv, int nb,
+                                           int b, int d, int ragged);
+
+/* Dense attention of each request's newest tokens over its whole paged cache.
+ * q [tokens, Hq, D] (q_stride elements from token to token): request r's rows
+ * are [starts[r], starts[r + 1]), or row r alone with starts null (tokens =
+ * requests); they are its last tokens, the final one at position n_r - 1 of its
+ * n_r cached tokens.  A row at position p sees the keys [lo, hi):
+ *   lo = max(0, first[t], p - window + 1)   (first [tokens] may be null; window 0: none)
+ *   hi = max(p + 1, min(prefix[r], n_r))    (prefix [R] may be null)
+ * with scores softcap * tanh(scale q.k / softcap) (softcap 0: scale q.k) minus
+ * slopes[h] * |p - key| (slopes [Hq] may be null).  A row that sees no key is
+ * zero; keys that a row does not see, and keys on invalid pages, do not reach it,
+ * whatever they hold.  out [tokens, Hq, D] has the pages' type; its rows of
+ * no request are left as they are, or zeroed with fill != 0.  ragged (of the
+ * workspace query) says whether starts is given.  Shapes: FP16 / BF16, D in
+ * {64, 128, 256}, B a multiple of 16, scale > 0. */
+int stk_paged_attention(const void* q, int64_t q_stride, int dtype, int tokens, int requests,
+                        int hq, int hkv, int nb, int b, int d, int pages, const void* k_pages,
+                        const void* v_pages, const int32_t* block_table, const int32_t* nblocks,
+                        const int32_t* ntokens, const int32_t* starts, float scale,
+                        float softcap, const float* slopes, int window, const int32_t* prefix,
+                        const int32_t* first, void* out, int fill, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+size_t stk_paged_shared_workspace_bytes(int requests, int ngroups, int hq, int hkv, int nb, int b,
+                                        int d);
+
+/* stk_paged_attention of one token per request where requests share leading
+ * blocks: requests groups[i] .. groups[i + 1] - 1 (groups [ngroups + 1], not
+ * decreasing) hold the same pages in the first shared[i] blocks of their table rows.
+ * Those blocks are read once per group, through its first request's row, the
+ * others per request, and the parts joined.  Requests of no group share nothing. */
+int stk_paged_shared_attention(const void* q, int64_t q_stride, int dtype, int requests, int hq,
+                               int hkv, int nb, int b, int d, int pages, const void* k_pages,
+                               const void* v_pages, const int32_t* block_table,
+                               const int32_t* nblocks, const int32_t* ntokens,
+                               const int32_t* groups, const int32_t* shared, int ngroups,
+                               float scale, float softcap, const float* slopes, int window,
+                               const int32_t* first, void* out, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
 /* stk_speculative_step over a paged batch (union_mode: repair_union). */
 int stk_paged_step(const void* q, const void* k_pages, const void* v_pages, int dtype,
                    int requests, int hq, int hkv, int nb, int b, int d, int pages,

@@ -1,0 +1,458 @@
+// Dense attention over the paged cache: the C entry points, the list of row
+// tiles (k_plan), and the joins of split items (k_join_tiles, k_join_rows).
+#include "dense_decode.hpp"
+
+namespace stk {
+
+constexpr int kPlanThreads = 1024;
+
+// Lists the row tiles: one workgroup.  Within a sequence the last rows, which see
+// the most keys, come first.
+__global__ __launch_bounds__(kPlanThreads) void k_plan(DenseArgs a, Plan pl, int tk) {
+  __shared__ int s_a[kPlanThreads / STK_WAVE];
+  const int tid = threadIdx.x, ns = sequences(a);
+  int base = 0;
+  for (int q0 = 0; q0 < ns; q0 += kPlanThreads) {
+    const int q = q0 + tid;
+    int s0 = 0, s1 = 0, sum;
+    if (q < ns) seq_rows(a, q, s0, s1);
+    const int rt = (int)(((int64_t)(s1 - s0) * a.g + kDenseRows - 1) / kDenseRows);
+    __syncthreads();
+    const int before = base + block_excl_scan1(rt, s_a, &sum);
+    if (q < ns) pl.base[q] = before;
+    base += sum;
+  }
+  if (tid == 0) pl.base[ns] = base;
+  __syncthreads();                       // the workgroup's own stores are read back
+  const int rt = min(base, pl.limit);
+  int cum = 0;
+  for (int i0 = 0; i0 < rt; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    Tile x{};
+    int n = 0, sum;
+    if (i < rt) {
+      int lo = 0, hi = ns - 1;           // last sequence that begins at or before tile i
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (pl.base[mid] <= i) lo = mid;
+        else hi = mid - 1;
+      }
+      int s0, s1;
+      seq_rows(a, lo, s0, s1);
+      x.seq = lo;
+      x.tile = pl.base[lo + 1] - 1 - i;
+      const int64_t row0 = (int64_t)x.tile * kDenseRows;
+      const int64_t row1 = min(row0 + kDenseRows, (int64_t)(s1 - s0) * a.g) - 1;
+      const int t0 = s0 + (int)(row0 / a.g), t1 = s0 + (int)(row1 / a.g);
+      x.klo = 0x7fffffff;
+      x.khi = 0;
+      x.max_lo = 0;
+      x.min_hi = 0x7fffffff;
+      // without per-token starts the spans of a request's tokens only move up
+      const int step = a.groups || a.first ? 1 : max(1, t1 - t0);
+      for (int t = t0; t <= t1; t += step) {
+        int p;
+        const Span s = seq_span(a, lo, s0, s1, t, p);
+        if (s.hi > s.lo) {
+          x.klo = min(x.klo, s.lo);
+          x.khi = max(x.khi, s.hi);
+          x.max_lo = max(x.max_lo, s.lo);
+          x.min_hi = min(x.min_hi, s.hi);
+        } else {
+          x.min_hi = 0;
+          // rows after this one may still see keys from their own lower end on
+          if (step > 1) x.klo = min(x.klo, s.lo);
+        }
+      }
+      if (x.khi <= x.klo) x.klo = x.khi = 0;
+      x.kstart = x.klo & ~15;
+      n = max(1, (x.khi - x.kstart + tk - 1) / tk);
+    }
+    __syncthreads();
+    x.cum = cum + block_excl_scan1(n, s_a, &sum);
+    if (i < rt) pl.tiles[i] = x;
+    cum += sum;
+  }
+  if (tid == 0) {
+    pl.head[0] = cum;
+    pl.head[1] = rt;
+  }
+}
+
+// Rows of the tiles whose units were dealt to several workgroups.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_join_tiles(DenseArgs a, Plan pl, Parts split, int launched) {
+  const int per = pl.head[0], ntiles = pl.head[1];
+  const int kvh = (int)blockIdx.x / pl.limit, it = (int)blockIdx.x % pl.limit;
+  if (it >= ntiles) return;
+  const Tile t = pl.tiles[it];
+  const int64_t total = (int64_t)per * a.hkv, first = (int64_t)kvh * per + t.cum;
+  const int n = (it + 1 < ntiles ? pl.tiles[it + 1].cum : per) - t.cum;
+  const int grid = split_grid(total, launched);
+  const int w0 = wg_of(total, first, grid), w1 = wg_of(total, first + n - 1, grid);
+  if (w0 == w1) return;
+  int s0, s1;
+  seq_rows(a, t.seq, s0, s1);
+  const int64_t row0 = (int64_t)t.tile * kDenseRows;
+  const int nrow = (int)min((int64_t)kDenseRows, (int64_t)(s1 - s0) * a.g - row0);
+  for (int x = threadIdx.x; x < nrow * (D / 4); x += 256) {
+    const int row = x / (D / 4), dc = x % (D / 4);
+    float m = -INFINITY, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int w = w0; w <= w1; ++w) {
+      const int64_t pr = (2 * (int64_t)w + (w == w0 ? 1 : 0)) * kDenseRows + row;
+      const float mi = split.m[pr], li = split.l[pr], mx = fmaxf(m, mi);
+      const f32x4 oi = *reinterpret_cast<const f32x4*>(split.o + pr * D + 4 * dc);
+      const float f = part_weight(m, mx), fi = part_weight(mi, mx);
+      m = mx;
+      l = l * f + li * fi;
+      o = o * f + oi * fi;
+    }
+    const int tok = s0 + (int)((row0 + row) / a.g), head = kvh * a.g + (int)((row0 + row) % a.g);
+    store_out<T>(a.out + ((int64_t)tok * a.hq + head) * D + 4 * dc, o, l);
+  }
+}
+
+// One (request, query head) of a decode batch: the parts of its own keys, and
+// with groups those of the shared keys.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Parts whole,
+                                                   int launched, Plan pl, Parts psplit,
+                                                   Parts pwhole, int plaunched) {
+  constexpr int CH = D / 4, NP = 256 / CH;       // 4-wide columns, parts in flight
+  __shared__ float s_m[NP], s_l[NP];
+  __shared__ f32x4 s_o[NP][CH];
+  const int r = (int)blockIdx.x / a.hq, head = (int)blockIdx.x % a.hq;
+  const int kvh = head / a.g, gi = head % a.g, nc = decode_chunks(a);
+  const int item = kvh * nc + gi / kDecodeRows, hrow = gi % kDecodeRows;
+  const DecodePlace at = decode_place<true>(a, r, 0);
+  const DecodeSpan sp = decode_span(a, r);
+  const int first = at.base + item * sp.n, grid = split_grid(at.total, launched);
+  const int w0 = wg_of(at.total, first, grid), w1 = wg_of(at.total, first + sp.n - 1, grid);
+  const int ns = w1 - w0 + 1;
+  int np = 0, v0 = 0, rr = 0;
+  int64_t pslot = 0;
+  if (a.groups) {
+    const int g = group_of(a, r);
+    if (g >= 0) {
+      int s0, s1;
+      seq_rows(a, g, s0, s1);
+      const int64_t idx = (int64_t)(r - s0) * a.g + gi;
+      const int tile = (int)(idx / kDenseRows), it = pl.base[g + 1] - 1 - tile;
+      rr = (int)(idx % kDenseRows);
+      const int per = pl.head[0], ntiles = pl.head[1];
+      const int cum = pl.tiles[it].cum;
+      const int n = (it + 1 < ntiles ? pl.tiles[it + 1].cum : per) - cum;
+      const int64_t total = (int64_t)per * a.hkv, pf = (int64_t)kvh * per + cum;
+      const int pgrid = split_grid(total, plaunched);
+      v0 = wg_of(total, pf, pgrid);
+      np = wg_of(total, pf + n - 1, pgrid) - v0 + 1;
+      pslot = (int64_t)kvh * ntiles + it;
+    }
+  } else if (ns == 1) {
+    return;                                      // finished by its workgroup
+  }
+  const int dc = threadIdx.x % CH, grp = threadIdx.x / CH;
+  float m = -INFINITY, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int i = grp; i < ns + np; i += NP) {
+    const float *pm, *pl_, *po;
+    int64_t pr;
+    if (i < ns) {
+      const Parts& from = ns == 1 ? whole : split;
+      pr = (ns == 1 ? (int64_t)r * a.hkv * nc + item : 2 * (int64_t)(w0 + i) + (i == 0 ? 1 : 0)) *
+               kDecodeRows + hrow;
+      pm = from.m; pl_ = from.l; po = from.o;
+    } else {
+      const int q = i - ns;
+      const Parts& from = np == 1 ? pwhole : psplit;
+      pr = (np == 1 ? pslot : 2 * (int64_t)(v0 + q) + (q == 0 ? 1 : 0)) * kDenseRows + rr;
+      pm = from.m; pl_ = from.l; po = from.o;
+    }
+    const float mi = pm[pr], li = pl_[pr], mx = fmaxf(m, mi);
+    const f32x4 oi = *reinterpret_cast<const f32x4*>(po + pr * D + 4 * dc);
+    const float f = part_weight(m, mx), fi = part_weight(mi, mx);
+    m = mx;
+    l = l * f + li * fi;
+    o = o * f + oi * fi;
+  }
+  if (dc == 0) {
+    s_m[grp] = m;
+    s_l[grp] = l;
+  }
+  s_o[grp][dc] = o;
+  __syncthreads();
+  if (grp == 0) {
+    for (int i = 1; i < NP; ++i) {
+      const float mi = s_m[i], mx = fmaxf(m, mi);
+      const float f = part_weight(m, mx), fi = part_weight(mi, mx);
+      m = mx;
+      l = l * f + s_l[i] * fi;
+      o = o * f + s_o[i][dc] * fi;
+    }
+    store_out<T>(a.out + ((int64_t)r * a.hq + head) * D + 4 * dc, o, l);
+  }
+}
+
+// ------------------------------------------------------------------ host
+
+constexpr int kFill = 512;          // workgroups that fill the device: two per CU
+
+struct DenseShape {
+  int tokens, requests, hq, hkv, nb, b, d, ngroups;
+  bool ragged;
+};
+
+static StkCheck check_dense(const DenseShape& s, int dtype, int pages) {
+  if (dtype != DT_F16 && dtype != DT_BF16) return {false, "the cache must be FP16 or BF16"};
+  if (s.tokens < 0 || s.requests < 1 || s.nb < 1 || pages < 1) return {false, "bad shape"};
+  StkCheck c = stk_check_kv(dtype, s.hq, s.hkv, s.nb, s.b, s.d);
+  if (!c.ok) return c;
+  if (s.hq < 1) return {false, "expected nonempty shapes"};
+  if (s.d != 64 && s.d != 128 && s.d != 256)
+    return {false, "head dimension must be 64, 128 or 256"};
+  if (s.b % 16) return {false, "the block size must be a multiple of 16"};
+  const int64_t keys = (int64_t)s.nb * s.b;
+  if (keys > (1ll << 30) || keys * s.b > (1ll << 40) || (int64_t)pages * s.b > 0x7fffffff)
+    return {false, "cache too large"};
+  return {true, ""};
+}
+
+static int64_t decode_units(const DenseShape& s) {
+  const int g = s.hq / s.hkv, nc = (g + kDecodeRows - 1) / kDecodeRows;
+  return (int64_t)s.requests * s.hkv * nc * (((int64_t)s.nb * s.b + kUnit - 1) / kUnit + 1);
+}
+static int decode_grid(const DenseShape& s) {
+  const int64_t u = decode_units(s);
+  return u < kFill ? (int)u : kFill;
+}
+static int64_t tile_limit(const DenseShape& s) {
+  const int ns = s.ngroups ? s.ngroups : s.requests;
+  const int64_t rows = (int64_t)(s.ngroups ? s.requests : s.tokens) * (s.hq / s.hkv);
+  return rows / kDenseRows + ns;
+}
+static int64_t prefill_units(const DenseShape& s) {
+  const int tk = s.d == 256 ? 32 : 64;
+  return tile_limit(s) * s.hkv * (((int64_t)s.nb * s.b + tk - 1) / tk + 1);
+}
+// Tiles that fill the device several times over need no splitting.
+constexpr int64_t kDirectTiles = 4 * kFill;
+static bool prefill_direct(const DenseShape& s) {
+  return !s.ngroups && tile_limit(s) * s.hkv >= kDirectTiles;
+}
+static int prefill_grid(const DenseShape& s) {
+  if (prefill_direct(s)) return (int)(tile_limit(s) * s.hkv);
+  const int fill = s.d == 256 ? kFill / 2 : kFill;
+  const int64_t u = prefill_units(s);
+  return u < fill ? (int)u : fill;
+}
+
+static size_t parts_bytes(int64_t slots, int rows, int d) {
+  return 2 * stk_align((size_t)slots * rows * sizeof(float)) +
+         stk_align((size_t)slots * rows * d * sizeof(float));
+}
+static Parts take_parts(Carve& c, int64_t slots, int rows, int d) {
+  Parts p;
+  p.m = c.take<float>((size_t)slots * rows);
+  p.l = c.take<float>((size_t)slots * rows);
+  p.o = c.take<float>((size_t)slots * rows * d);
+  return p;
+}
+static size_t plan_bytes(const DenseShape& s) {
+  const int ns = s.ngroups ? s.ngroups : s.requests;
+  return stk_align(2 * sizeof(int32_t)) + stk_align((ns + 1) * sizeof(int32_t)) +
+         stk_align((size_t)tile_limit(s) * sizeof(Tile));
+}
+static Plan take_plan(Carve& c, const DenseShape& s) {
+  const int ns = s.ngroups ? s.ngroups : s.requests;
+  Plan p;
+  p.head = c.take<int32_t>(2);
+  p.base = c.take<int32_t>(ns + 1);
+  p.limit = (int)tile_limit(s);
+  p.tiles = c.take<Tile>(p.limit);
+  return p;
+}
+
+static size_t dense_bytes(const DenseShape& s) {
+  const int nc = (s.hq / s.hkv + kDecodeRows - 1) / kDecodeRows;
+  size_t x = 0;
+  if (!s.ragged) {
+    x += parts_bytes(2 * (int64_t)decode_grid(s), kDecodeRows, s.d);
+    if (s.ngroups) x += parts_bytes((int64_t)s.requests * s.hkv * nc, kDecodeRows, s.d);
+  }
+  if (s.ragged || s.ngroups) {
+    x += plan_bytes(s);
+    if (!prefill_direct(s)) x += parts_bytes(2 * (int64_t)prefill_grid(s), kDenseRows, s.d);
+    if (s.ngroups) x += parts_bytes(tile_limit(s) * s.hkv, kDenseRows, s.d);
+  }
+  return x;
+}
+
+static int launch_plan(const DenseArgs& a, const Plan& p, int d, hipStream_t st) {
+  hipLaunchKernelGGL(k_plan, dim3(1), dim3(kPlanThreads), 0, st, a, p, d == 256 ? 32 : 64);
+  return stk_check_launch("k_plan");
+}
+
+template <typename T>
+static void launch_join_tiles(const DenseArgs& a, const Plan& p, const Parts& split, int grid,
+                              int d, hipStream_t st) {
+  const dim3 g((unsigned)(p.limit * a.hkv));
+  if (d == 64) hipLaunchKernelGGL((k_join_tiles<T, 64>), g, dim3(256), 0, st, a, p, split, grid);
+  else if (d == 128)
+    hipLaunchKernelGGL((k_join_tiles<T, 128>), g, dim3(256), 0, st, a, p, split, grid);
+  else hipLaunchKernelGGL((k_join_tiles<T, 256>), g, dim3(256), 0, st, a, p, split, grid);
+}
+
+template <typename T>
+static void launch_join_rows(const DenseArgs& a, const Parts& split, const Parts& whole, int grid,
+                             const Plan& p, const Parts& ps, const Parts& pw, int pgrid, int d,
+                             hipStream_t st) {
+  const dim3 g((unsigned)(a.requests * a.hq));
+#define STK_JOIN(D) \
+  hipLaunchKernelGGL((k_join_rows<T, D>), g, dim3(256), 0, st, a, split, whole, grid, p, ps, pw, pgrid)
+  if (d == 64) STK_JOIN(64);
+  else if (d == 128) STK_JOIN(128);
+  else STK_JOIN(256);
+#undef STK_JOIN
+}
+
+template <typename T>
+static int run_dense(const DenseShape& s, DenseArgs a, int mode, void* workspace, hipStream_t st) {
+  Carve c(workspace);
+  const Parts none{nullptr, nullptr, nullptr};
+  if (s.ragged) {
+    const Plan p = take_plan(c, s);
+    const bool direct = prefill_direct(s);
+    const int grid = prefill_grid(s);
+    const Parts split = direct ? none : take_parts(c, 2 * (int64_t)grid, kDenseRows, s.d);
+    int rc = launch_plan(a, p, s.d, st);
+    if (rc) return rc;
+    rc = launch_prefill<T>(s.d, mode, a, p, split, none, grid, direct, st);
+    if (rc || direct) return rc;
+    launch_join_tiles<T>(a, p, split, grid, s.d, st);
+    return stk_check_launch("k_join_tiles");
+  }
+  const int nc = (a.g + kDecodeRows - 1) / kDecodeRows;
+  const int grid = decode_grid(s);
+  const Parts split = take_parts(c, 2 * (int64_t)grid, kDecodeRows, s.d);
+  Parts whole = none, ps = none, pw = none;
+  Plan p{};
+  int pgrid = 0;
+  if (s.ngroups) {
+    whole = take_parts(c, (int64_t)s.requests * s.hkv * nc, kDecodeRows, s.d);
+    p = take_plan(c, s);
+    pgrid = prefill_grid(s);
+    ps = take_parts(c, 2 * (int64_t)pgrid, kDenseRows, s.d);
+    pw = take_parts(c, tile_limit(s) * s.hkv, kDenseRows, s.d);
+    int rc = launch_plan(a, p, s.d, st);
+    if (rc) return rc;
+    rc = launch_prefill<T>(s.d, mode, a, p, ps, pw, pgrid, false, st);
+    if (rc) return rc;
+  }
+  int rc = launch_decode<T>(s.d, mode, a, split, whole, grid, st);
+  if (rc) return rc;
+  launch_join_rows<T>(a, split, whole, grid, p, ps, pw, pgrid, s.d, st);
+  return stk_check_launch("k_join_rows");
+}
+
+static int dense(const DenseShape& s, const void* q, int64_t q_stride, int dtype, int pages,
+                 const void* k_pages, const void* v_pages, const int32_t* table,
+                 const int32_t* nblocks, const int32_t* ntokens, const int32_t* starts,
+                 const int32_t* groups, const int32_t* shared, float scale, float softcap,
+                 const float* slopes, int window, const int32_t* prefix, const int32_t* first,
+                 void* out, int fill, void* workspace, size_t workspace_bytes, void* stream) {
+  STK_REQUIRE(check_dense(s, dtype, pages));
+  STK_REQUIRE(s.ragged || s.tokens == s.requests, "expected one query token per request");
+  STK_REQUIRE(s.tokens == 0 || (q && out), "null pointer");
+  STK_REQUIRE(k_pages && v_pages && table && nblocks, "null pointer");
+  STK_REQUIRE(scale > 0.f && scale <= 3.402823466e38f, "scale must be positive and finite");
+  STK_REQUIRE(softcap >= 0.f && softcap <= 3.402823466e38f,
+              "softcap must be finite, 0 for none");
+  STK_REQUIRE(window >= 0, "window must be at least 0 (0: none)");
+  STK_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) |
+                reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) &
+               15) == 0 && q_stride % 8 == 0 && q_stride >= 0,
+              "rows must be 16-byte aligned");
+  STK_REQUIRE(decode_units(s) <= 0x7fffffff && (int64_t)s.requests * s.hq <= 0x7fffffff &&
+                  prefill_units(s) <= 0x7fffffff,
+              "batch too large");
+  STK_REQUIRE(workspace && workspace_bytes >= dense_bytes(s), "workspace too small");
+  STK_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+              "the workspace must be 16-byte aligned");
+  if (s.tokens == 0) return STK_OK;
+  const double log2e = 1.4426950408889634;
+  DenseArgs a{};
+  a.q = static_cast<const uint16_t*>(q); a.qs = q_stride;
+  a.out = static_cast<uint16_t*>(out);
+  a.kp = static_cast<const uint16_t*>(k_pages); a.vp = static_cast<const uint16_t*>(v_pages);
+  a.table = table; a.nblocks = nblocks; a.ntokens = ntokens; a.starts = starts;
+  a.t = s.tokens; a.requests = s.requests; a.hq = s.hq; a.hkv = s.hkv; a.g = s.hq / s.hkv;
+  a.nb = s.nb; a.b = s.b; a.pages = pages;
+  a.bdiv = (1ull << 32) / (uint64_t)(s.b / 16) + 1;
+  a.c = (float)(scale * log2e);
+  if (softcap > 0.f) {
+    a.cap_in = (float)(2.0 * log2e * scale / softcap);
+    a.cap_out = (float)(softcap * log2e);
+  }
+  a.slopes = slopes; a.window = window; a.prefix = prefix; a.first = first;
+  a.groups = groups; a.shared = shared; a.ngroups = s.ngroups; a.fill = fill;
+  const int mode = (softcap > 0.f ? 1 : 0) | (slopes ? 2 : 0);
+  hipStream_t st = (hipStream_t)stream;
+  return dtype == DT_BF16 ? run_dense<bf16s>(s, a, mode, workspace, st)
+                          : run_dense<f16s>(s, a, mode, workspace, st);
+}
+
+}  // namespace stk
+
+using namespace stk;
+
+extern "C" {
+
+STK_API size_t stk_paged_attention_workspace_bytes(int tokens, int requests, int hq, int hkv,
+                                                   int nb, int b, int d, int ragged) {
+  if (tokens <= 0 || requests <= 0 || hq <= 0 || hkv <= 0 || nb <= 0 || b <= 0 || d <= 0 ||
+      hq % hkv)
+    return 0;
+  return dense_bytes({tokens, requests, hq, hkv, nb, b, d, 0, ragged != 0});
+}
+
+STK_API int stk_paged_attention(const void* q, int64_t q_stride, int dtype, int tokens,
+                                int requests, int hq, int hkv, int nb, int b, int d, int pages,
+                                const void* k_pages, const void* v_pages,
+                                const int32_t* block_table, const int32_t* nblocks,
+                                const int32_t* ntokens, const int32_t* starts, float scale,
+                                float softcap, const float* slopes, int window,
+                                const int32_t* prefix, const int32_t* first, void* out, int fill,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  return dense({tokens, requests, hq, hkv, nb, b, d, 0, starts != nullptr}, q, q_stride, dtype,
+               pages, k_pages, v_pages, block_table, nblocks, ntokens, starts, nullptr, nullptr,
+               scale, softcap, slopes, window, prefix, first, out, fill, workspace,
+               workspace_bytes, stream);
+}
+
+STK_API size_t stk_paged_shared_workspace_bytes(int requests, int ngroups, int hq, int hkv, int nb,
+                                                int b, int d) {
+  if (requests <= 0 || ngroups <= 0 || hq <= 0 || hkv <= 0 || nb <= 0 || b <= 0 || d <= 0 ||
+      hq % hkv)
+    return 0;
+  return dense_bytes({requests, requests, hq, hkv, nb, b, d, ngroups, false});
+}
+
+STK_API int stk_paged_shared_attention(const void* q, int64_t q_stride, int dtype, int requests,
+                                       int hq, int hkv, int nb, int b, int d, int pages,
+                                       const void* k_pages, const void* v_pages,
+                                       const int32_t* block_table, const int32_t* nblocks,
+                                       const int32_t* ntokens, const int32_t* groups,
+                                       const int32_t* shared, int ngroups, float scale,
+                                       float softcap, const float* slopes, int window,
+                                       const int32_t* first, void* out, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+  STK_REQUIRE(groups && shared, "null pointer");
+  STK_REQUIRE(ngroups >= 1 && ngroups <= requests, "expected 1 to R groups");
+  return dense({requests, requests, hq, hkv, nb, b, d, ngroups, false}, q, q_stride, dtype, pages,
+               k_pages, v_pages, block_table, nblocks, ntokens, nullptr, groups, shared, scale,
+               softcap, slopes, window, nullptr, first, out, 0, workspace, workspace_bytes,
+               stream);
+}
+
+}  // extern "C"

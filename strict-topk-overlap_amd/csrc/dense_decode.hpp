@@ -1,0 +1,312 @@
+// Dense attention of single tokens over the paged cache.
+//
+// An item is one request's KV head with up to 16 of its query heads; its keys
+// are cut into units of kUnit keys, and the units of all items, laid end to end,
+// are dealt evenly over one grid that fills the device: a ragged batch, or one long
+// request, keeps every CU busy to the end.  A workgroup walks its run of units
+// item by item.  Items that lie whole in one workgroup are finished there; the
+// parts of the others are joined by k_join.  Nothing of this needs the lengths on
+// the host.
+//
+// Within a workgroup the four waves take a quarter of the keys each and share
+// nothing until the item ends.  A wave's tile is 32 keys:
+//   S[key, head] = K Q^T  (16x16x32, K straight from global memory to registers,
+//                          in the operand's own layout),
+//   O^T[dim, head] += V^T P^T  (V through the wave's own LDS, read transposed).
+// Lane (n, g) of S holds keys 4g .. 4g + 3 of both 16-key halves for head n, and
+// the order of the keys within the second product is free: taking {4g .. 4g + 3,
+// 16 + 4g .. 16 + 4g + 3} as its eight, P never leaves its lane.
+// The next tile's K and V are in flight while a tile is worked on.
+//
+// Bound by HBM: every key and value is read once (per 16 query heads of its KV head).
+#pragma once
+
+#include "dense.hpp"
+
+namespace stk {
+
+// Decode work of request r: its visible keys, cut into n units from lo16.
+struct DecodeSpan { int lo, hi, lo16, n; };
+
+__device__ __forceinline__ DecodeSpan decode_span(const DenseArgs& a, int r) {
+  const int n = tokens_of(a, r);
+  const Span s = span_of(a, r, r, n - 1, n);
+  DecodeSpan d{s.lo, s.hi, 0, 1};
+  if (a.groups) {
+    const int g = group_of(a, r);
+    if (g >= 0) d.lo = max(d.lo, shared_of(a, g));
+  }
+  d.lo16 = d.lo & ~15;
+  if (d.hi > d.lo) d.n = (d.hi - d.lo16 + kUnit - 1) / kUnit;
+  return d;
+}
+
+__device__ __forceinline__ int decode_chunks(const DenseArgs& a) {
+  return (a.g + kDecodeRows - 1) / kDecodeRows;
+}
+
+// The requests' units laid end to end: how many there are, a request, and the
+// units before it.  BY_REQUEST: request `want`; else the request that holds
+// the first unit of workgroup `want` (past the last one with work: any).
+struct DecodePlace { int total, base, r; };
+
+template <bool BY_REQUEST>
+__device__ __forceinline__ DecodePlace decode_place(const DenseArgs& a, int want, int launched) {
+  __shared__ int s_tmp[4], s_at[2];
+  const int per = a.hkv * decode_chunks(a);
+  int total = 0, c0 = 0, b0 = 0, sum0 = 0;
+  for (int r0 = 0; r0 < a.requests; r0 += 256) {
+    const int r = r0 + (int)threadIdx.x;
+    const int c = r < a.requests ? decode_span(a, r).n * per : 0;
+    int sum;
+    __syncthreads();
+    const int before = total + block_excl_scan1(c, s_tmp, &sum);
+    if (BY_REQUEST && r == want) s_at[0] = before;
+    if (r0 == 0) {
+      c0 = c;
+      b0 = before;
+      sum0 = sum;
+    }
+    total += sum;
+  }
+  if (!BY_REQUEST) {
+    const int u = (int)unit_at(total, want, split_grid(total, launched));
+    int base = 0;
+    for (int r0 = 0; r0 < a.requests; r0 += 256) {
+      const int r = r0 + (int)threadIdx.x;
+      int c = c0, before = b0, sum = sum0;
+      if (r0 > 0) {
+        c = r < a.requests ? decode_span(a, r).n * per : 0;
+        __syncthreads();
+        before = base + block_excl_scan1(c, s_tmp, &sum);
+      }
+      if (u >= before && u < before + c) {
+        s_at[0] = before;
+        s_at[1] = r;
+      }
+      base += sum;
+    }
+  }
+  __syncthreads();
+  DecodePlace p{total, s_at[0], BY_REQUEST ? want : s_at[1]};
+  p.base = __builtin_amdgcn_readfirstlane(p.base);
+  p.r = __builtin_amdgcn_readfirstlane(p.r);
+  return p;
+}
+
+template <typename T, int D, int MODE>
+__global__ __launch_bounds__(256, 2) void k_decode(DenseArgs a, Parts split, Parts whole) {
+  constexpr int KS = D / 32;            // QK steps
+  constexpr int DB = D / 16;            // output blocks
+  constexpr int VN = D / 16;            // 16-byte chunks of a V tile per lane
+  constexpr int CPR = D / 8;            // chunks per row
+  constexpr int RPI = STK_WAVE / CPR;   // rows per load instruction
+  __shared__ __attribute__((aligned(16))) uint16_t s_v[4][32 * D];
+  __shared__ float s_m[4][16], s_l[4][16];
+  const int lane = lane_id(), w = wave_id();
+  const int n16 = lane & 15, kg = lane >> 4;
+  const int nc = decode_chunks(a);
+  const DecodePlace at = decode_place<false>(a, (int)blockIdx.x, (int)gridDim.x);
+  const int grid = split_grid(at.total, (int)gridDim.x);
+  if ((int)blockIdx.x >= grid) return;
+  int u = (int)unit_at(at.total, (int)blockIdx.x, grid);
+  const int u1 = (int)unit_at(at.total, (int)blockIdx.x + 1, grid);
+  int r = at.r, base = at.base;
+  // V tile in LDS: row-major, 32-byte blocks swizzled so that the 16 rows of a
+  // transposed read spread over all banks
+  auto fsw = [](int row) { return D == 64 ? (row >> 1) & 3 : row & 7; };
+  uint16_t* vt = s_v[w];
+  int vw[VN], va[DB];
+#pragma unroll
+  for (int i = 0; i < VN; ++i) {
+    const int row = i * RPI + lane / CPR, ch = lane % CPR;
+    vw[i] = row * D + ((((ch >> 1) ^ fsw(row)) << 1) | (ch & 1)) * 8;
+  }
+#pragma unroll
+  for (int db = 0; db < DB; ++db) {
+    const int row = 4 * kg + (n16 >> 2);
+    va[db] = row * D + (db ^ fsw(row)) * 16 + 4 * (n16 & 3);
+  }
+  while (u < u1) {
+    DecodeSpan sp = decode_span(a, r);
+    sp.lo = __builtin_amdgcn_readfirstlane(sp.lo);
+    sp.hi = __builtin_amdgcn_readfirstlane(sp.hi);
+    sp.lo16 = __builtin_amdgcn_readfirstlane(sp.lo16);
+    sp.n = __builtin_amdgcn_readfirstlane(sp.n);
+    const int per = a.hkv * nc * sp.n;
+    if (u >= base + per) {
+      base += per;
+      ++r;
+      continue;
+    }
+    const int item = (u - base) / sp.n, j0 = (u - base) % sp.n;
+    const int j1 = min(sp.n, j0 + (u1 - u));
+    u += j1 - j0;
+    const int kvh = item / nc, h0 = kvh * a.g + (item % nc) * kDecodeRows;
+    const int gn = min(kDecodeRows, a.g - (item % nc) * kDecodeRows);
+    const int ka = sp.lo16 + j0 * kUnit;
+    const int kb = (int)min((int64_t)sp.lo16 + (int64_t)j1 * kUnit, (int64_t)sp.hi);
+    const int32_t* row = a.table + ((int64_t)r * a.hkv + kvh) * a.nb;
+    // this head's query as the second operand: head n16, dims 32 s + 8 kg ..
+    u16x8 qf[KS];
+    const uint16_t* qp = a.q + (int64_t)r * a.qs + (int64_t)(h0 + min(n16, gn - 1)) * D + 8 * kg;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u16x8*>(qp + 32 * s);
+    float slope = 0.f;
+    if constexpr (MODE & 2) slope = a.slopes[h0 + min(n16, gn - 1)] * 1.44269504f;
+    float m = -INFINITY, l = 0.f;
+    f32x4 acc[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    const int nt = kb > ka ? (kb - ka + 31) / 32 : 0, tpw = (nt + 3) / 4;
+    const int ta = w * tpw, tb = min(nt, ta + tpw);
+    if (ta < tb) {
+      const int wk = ka + 32 * ta;                      // the wave's first key
+      auto window = [&](int i) {                        // rows of 64 runs of 16 keys
+        const int key = wk + 16 * (64 * i + lane);
+        const int x = pool_row(a, row, min(key, kb));
+        return key < kb ? x : -1;
+      };
+      int ent = window(0), nxt = window(1);
+      u16x8 kf[2][KS], vf[VN];
+      int r0, r1;
+      auto load = [&](int t) {
+        if (t > 0 && (t & 31) == 0) {
+          ent = nxt;
+          nxt = window(t / 32 + 1);
+        }
+        r0 = __builtin_amdgcn_readlane(ent, (2 * t) & 63);
+        r1 = __builtin_amdgcn_readlane(ent, (2 * t + 1) & 63);
+        const int64_t p0 = (int64_t)max(r0, 0) * D, p1 = (int64_t)max(r1, 0) * D;
+        const int ko = n16 * D + 8 * kg;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          kf[0][s] = *reinterpret_cast<const u16x8*>(a.kp + p0 + ko + 32 * s);
+          kf[1][s] = *reinterpret_cast<const u16x8*>(a.kp + p1 + ko + 32 * s);
+        }
+#pragma unroll
+        for (int i = 0; i < VN; ++i) {
+          const int vr = i * RPI;                       // rows vr .. vr + RPI - 1
+          vf[i] = *reinterpret_cast<const u16x8*>(
+              a.vp + (vr < 16 ? p0 : p1) + ((vr & 15) + lane / CPR) * D + 8 * (lane % CPR));
+        }
+      };
+      load(0);
+      const int cnt = tb - ta;
+      for (int t = 0; t < cnt; ++t) {
+        const int key0 = wk + 32 * t;
+        const bool full = key0 >= sp.lo && key0 + 32 <= kb && r0 >= 0 && r1 >= 0;
+        if (!full) {
+          // keys that are not seen: their values are not read as numbers
+#pragma unroll
+          for (int i = 0; i < VN; ++i) {
+            const int kr = i * RPI + lane / CPR, key = key0 + kr;
+            const bool ok = key >= sp.lo && key < kb && (kr < 16 ? r0 : r1) >= 0;
+            if (!ok) vf[i] = u16x8{};
+          }
+        }
+        const int rr0 = r0, rr1 = r1;
+#pragma unroll
+        for (int i = 0; i < VN; ++i) *reinterpret_cast<u16x8*>(vt + vw[i]) = vf[i];
+        f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          s0 = mma16<T>(kf[0][s], qf[s], s0);
+          s1 = mma16<T>(kf[1][s], qf[s], s1);
+        }
+        if (t + 1 < cnt) load(t + 1);
+        float x[8];
+        const float dist = (float)(sp.hi - 1 - key0 - 4 * kg);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = score2<MODE>(a, s0[i], slope, dist - (float)i);
+          x[4 + i] = score2<MODE>(a, s1[i], slope, dist - (float)(16 + i));
+        }
+        if (!full) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = key0 + 4 * kg + i;
+            x[i] = key >= sp.lo && key < kb && rr0 >= 0 ? x[i] : -INFINITY;
+            x[4 + i] = key + 16 >= sp.lo && key + 16 < kb && rr1 >= 0 ? x[4 + i] : -INFINITY;
+          }
+        }
+        const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                                fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        if (__any(top > m + kLazy)) {
+          float mx = fmaxf(top, m);
+          mx = fmaxf(mx, __shfl_xor(mx, 16));
+          mx = fmaxf(mx, __shfl_xor(mx, 32));
+          const float f = mx == m ? 1.f : __builtin_amdgcn_exp2f(m - mx);
+          m = mx;
+          l *= f;
+#pragma unroll
+          for (int i = 0; i < DB; ++i) acc[i] *= f;
+        }
+        const float ms = m == -INFINITY ? 0.f : m;
+        u16x8 p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float e = __builtin_amdgcn_exp2f(x[i] - ms);
+          l += e;
+          p[i] = to16<T>(e);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const u16x4 lo = lds_tr(vt + va[db]), hi = lds_tr(vt + va[db] + 16 * D);
+          acc[db] = mma16<T>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), p, acc[db]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    // the waves' states: V's LDS holds each wave's output rows
+    float* so = reinterpret_cast<float*>(vt);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+      *reinterpret_cast<f32x4*>(so + n16 * D + 16 * db + 4 * kg) = acc[db];
+    if (lane < 16) {
+      s_m[w][lane] = m;
+      s_l[w][lane] = l;
+    }
+    __syncthreads();
+    const bool all = j0 == 0 && j1 == sp.n;
+    const bool keep = all && !whole.m;                  // finished here
+    const Parts& to = all ? whole : split;
+    const int64_t slot = all ? (int64_t)r * a.hkv * nc + item
+                             : 2 * (int64_t)blockIdx.x + (j0 > 0 ? 0 : 1);
+    for (int x = threadIdx.x; x < gn * (D / 4); x += 256) {
+      const int h = x / (D / 4), dc = x % (D / 4);
+      float mx = s_m[0][h];
+#pragma unroll
+      for (int i = 1; i < 4; ++i) mx = fmaxf(mx, s_m[i][h]);
+      float sum = 0.f;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float mi = s_m[i][h];
+        const float f = part_weight(mi, mx);
+        sum += f * s_l[i][h];
+        o += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(s_v[i]) + h * D +
+                                                 4 * dc);
+      }
+      if (keep) {
+        store_out<T>(a.out + ((int64_t)r * a.hq + h0 + h) * D + 4 * dc, o, sum);
+      } else {
+        const int64_t pr = slot * kDecodeRows + h;
+        *reinterpret_cast<f32x4*>(to.o + pr * D + 4 * dc) = o;
+        if (dc == 0) {
+          to.m[pr] = mx;
+          to.l[pr] = sum;
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace stk

@@ -23,6 +23,7 @@ _lib = None
 
 P = ctypes.c_void_p
 I = ctypes.c_int
+L = ctypes.c_int64
 F = ctypes.c_float
 Z = ctypes.c_size_t
 
@@ -84,6 +85,14 @@ _SIGS = {
                             P, P, P, P, P, P, P, P, P, P, P, P, Z, P]),
     "stk_paged_workspace_bytes": (Z, [I, I, I]),
     "stk_paged_append": (I, [P, P, I, I, I, I, I, I, I, P, P, P, P, I, P, P, P, P, P]),
+    "stk_paged_extend": (I, [P, L, P, L, P, L, P, I, I, I, I, I, I, I, I, I, P, P, P, P, I, I, I,
+                             P, P, P, P, I, P, P, P, P]),
+    "stk_paged_attention_workspace_bytes": (Z, [I, I, I, I, I, I, I, I]),
+    "stk_paged_attention": (I, [P, L, I, I, I, I, I, I, I, I, I, P, P, P, P, P, P, F, F, P, I, P,
+                                P, P, I, P, Z, P]),
+    "stk_paged_shared_workspace_bytes": (Z, [I, I, I, I, I, I, I]),
+    "stk_paged_shared_attention": (I, [P, L, I, I, I, I, I, I, I, I, P, P, P, P, P, P, P, I, F, F,
+                                       P, I, P, P, P, Z, P]),
     "stk_paged_step": (I, [P, P, P, I, I, I, I, I, I, I, I, P, P, I, P, P, P, I, P, I, I,
                            P, P, P, P, P, P, Z, P]),
     "stk_paged_signed_step": (I, [P, P, P, I, I, I, I, I, I, I, I, P, P, I, P, P, P, I, P, I, I,

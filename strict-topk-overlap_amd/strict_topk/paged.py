@@ -170,6 +170,241 @@ def append(kv, k_new, v_new, positions):
     return kv
 
 
+def _device_call(device, name, *args):
+    """``_lib.call`` on the tensors' own device and its current stream."""
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, _lib.stream(device))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, _lib.stream(device))
+
+
+def _check_pool(kv, bounds):
+    """The pool's own tensors: their shapes, types, device and layout."""
+    if not isinstance(kv, PagedKV):
+        raise TypeError("kv must be a PagedKV")
+    if kv.k_pages.ndim != 3 or kv.v_pages.shape != kv.k_pages.shape or kv.block_table.ndim != 3:
+        raise ValueError("expected K/V pages [P,B,D] and a block table [R,Hkv,NB]")
+    if kv.k_pages.dtype not in (torch.float16, torch.bfloat16) or \
+            kv.v_pages.dtype != kv.k_pages.dtype:
+        raise ValueError("the pages must be FP16 or BF16, K and V alike")
+    if any(t.dtype != torch.int32 for t in (kv.block_table, kv.nblocks)) or \
+            kv.nblocks.shape != (kv.requests,):
+        raise ValueError("block_table [R,Hkv,NB] and nblocks [R] must be int32")
+    if kv.ntokens is not None and (kv.ntokens.dtype != torch.int32 or
+                                   kv.ntokens.shape != (kv.requests,)):
+        raise ValueError("ntokens must be int32 [R]")
+    ts = [kv.k_pages, kv.v_pages, kv.block_table, kv.nblocks]
+    if kv.ntokens is not None:
+        ts.append(kv.ntokens)
+    if bounds:
+        shape = (kv.pages, kv.dim)
+        if kv.lo_pages.shape != shape or kv.hi_pages.shape != shape or \
+                kv.hi_pages.dtype != kv.lo_pages.dtype:
+            raise ValueError("expected lo and hi pages [P,D] of one type")
+        ts += [kv.lo_pages, kv.hi_pages]
+    dev = kv.k_pages.device
+    if dev.type != "cuda" or any(t.device != dev or not t.is_contiguous() for t in ts):
+        raise ValueError("the pool's tensors must be contiguous and on one CUDA device")
+    return dev
+
+
+def _check_tokens(name, x, kv, heads):
+    """Rows [T, heads, D] of the pool's type, contiguous within a token, and the stride from
+    one token to the next."""
+    if x.ndim != 3 or x.shape[2] != kv.dim or (heads is not None and x.shape[1] != heads):
+        raise ValueError(f"expected {name}[T,{'Hq' if heads is None else 'Hkv'},D] matching "
+                         "the pool")
+    if x.dtype != kv.k_pages.dtype or x.device != kv.k_pages.device:
+        raise ValueError(f"{name} must have the pages' type and device")
+    t, h, d = x.shape
+    if t and h and (x.stride(2) != 1 or (h > 1 and x.stride(1) != d) or
+                    (t > 1 and (x.stride(0) < h * d or x.stride(0) % 8))):
+        raise ValueError(f"{name} must be contiguous within a token, tokens a multiple of 8 "
+                         "elements apart")
+    return x.stride(0) if t > 1 else h * d
+
+
+def _check_ints(name, x, n, device):
+    if x.dtype != torch.int32 or x.shape != (n,):
+        raise ValueError(f"expected int32 {name}[{n}]")
+    if x.device != device or not x.is_contiguous():
+        raise ValueError(f"{name} must be contiguous and on the pool's device")
+
+
+def _overlap(a, b):
+    """Whether two contiguous tensors share memory."""
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    return a0 < b0 + b.numel() * b.element_size() and b0 < a0 + a.numel() * a.element_size()
+
+
+def extend(kv, k_new, v_new, starts, positions, cos=None, sin=None, q=None, interleaved=False):
+    """Write the new tokens of a ragged batch into the cache, in place and in one launch.
+
+    k_new, v_new [T, Hkv, D] hold request r's new tokens in rows starts[r] ..
+    starts[r + 1] - 1 (starts int32 [R + 1], not decreasing); the first goes
+    to token position positions[r] (int32 [R], not kv.ntokens itself).  With
+    ``cos`` and ``sin`` (float32 [L, rot / 2], L >= NB * B, rot a multiple of
+    16 up to D) the keys are rotated to their positions: element i of the first rot with i
+    + rot / 2, or neighbours with ``interleaved``.  ``q`` [T, Hq, D] is rotated
+    the same way into a new tensor, which is returned (None without q); its rows
+    behind the last request are zero.  Touched pages' lo/hi take in the keys as
+    stored (a block whose first new token has offset 0 starts them over), and
+    nblocks and ntokens become each request's end.
+
+    Tokens past the table's width, and those whose block has no valid page, are
+    not written, and their request keeps its counts.  Tokens may lie
+    apart (views of one fused projection), heads and dims must not.  All
+    lengths stay on the device, so a captured graph follows them."""
+    dev = _check_pool(kv, True)
+    r, hkv = kv.requests, kv.hkv
+    ks = _check_tokens("K_NEW", k_new, kv, hkv)
+    vs = _check_tokens("V_NEW", v_new, kv, hkv)
+    t = k_new.shape[0]
+    if v_new.shape[0] != t:
+        raise ValueError("K_NEW and V_NEW must have the same tokens")
+    _check_ints("starts", starts, r + 1, dev)
+    _check_ints("positions", positions, r, dev)
+    if any(_overlap(positions, x) for x in (kv.ntokens, kv.nblocks) if x is not None):
+        raise ValueError("positions must not share memory with the cache's counts")
+    rows = rot = 0
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    if cos is not None:
+        if cos.ndim != 2 or sin.shape != cos.shape or cos.dtype != torch.float32 or \
+                sin.dtype != torch.float32:
+            raise ValueError("expected float32 cos and sin [L, rot / 2]")
+        if any(x.device != dev or not x.is_contiguous() for x in (cos, sin)):
+            raise ValueError("cos and sin must be contiguous and on the pool's device")
+        rows, rot = cos.shape[0], 2 * cos.shape[1]
+    hq, qs, out = 0, 0, None
+    if q is not None:
+        if cos is None:
+            raise ValueError("q needs cos and sin")
+        qs = _check_tokens("Q", q, kv, None)
+        hq = q.shape[1]
+        if q.shape[0] != t or hq < 1:
+            raise ValueError("Q must have K_NEW's tokens and at least one head")
+        out = torch.empty((t, hq, kv.dim), dtype=q.dtype, device=dev)
+    _device_call(dev, "stk_paged_extend", _lib.ptr(k_new), ks, _lib.ptr(v_new), vs, _lib.ptr(q), qs,
+                 _lib.ptr(out), _lib.dtype_code(k_new), t, r, hq, hkv, kv.width, kv.block, kv.dim,
+                 kv.pages, _lib.ptr(starts), _lib.ptr(positions), _lib.ptr(cos), _lib.ptr(sin),
+                 rows, rot, 1 if interleaved else 0, _lib.ptr(kv.k_pages), _lib.ptr(kv.v_pages),
+                 _lib.ptr(kv.lo_pages), _lib.ptr(kv.hi_pages),
+                 _lib.bounds_code(kv.lo_pages, kv.k_pages), _lib.ptr(kv.block_table),
+                 _lib.ptr(kv.nblocks), _lib.ptr(kv.ntokens))
+    return out
+
+
+def _dense_args(q, kv, scale, softcap, slopes, window, first, out):
+    """The checks that ``attention`` and ``shared_attention`` have in common."""
+    dev = _check_pool(kv, False)
+    qs = _check_tokens("Q", q, kv, None)
+    t, hq, d = q.shape
+    if hq < 1 or hq % kv.hkv:
+        raise ValueError("Hq must be divisible by Hkv")
+    scale = d ** -0.5 if scale is None else float(scale)
+    softcap = float(softcap or 0.0)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError("scale must be positive and finite")
+    if not 0.0 <= softcap < float("inf"):
+        raise ValueError("softcap must be finite and at least 0 (0: none)")
+    window = int(window or 0)
+    if not 0 <= window < 2 ** 31:
+        raise ValueError("window must be at least 0 (0: none)")
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (hq,) or
+                               slopes.device != dev or not slopes.is_contiguous()):
+        raise ValueError("slopes must be contiguous float32 [Hq] on the pool's device")
+    if first is not None:
+        _check_ints("first", first, t, dev)
+    if out is None:
+        res = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != dev or \
+                not out.is_contiguous():
+            raise ValueError("out must be contiguous, with Q's shape, type and device")
+        res = out
+    return dev, qs, t, hq, d, scale, softcap, window, res
+
+
+def attention(q, kv, starts=None, scale=None, softcap=0.0, slopes=None, window=0, prefix=None,
+              first=None, out=None):
+    """Dense attention of each request's newest tokens over its whole cache.
+
+    q [T, Hq, D]: rows starts[r] .. starts[r + 1] - 1 (starts int32 [R + 1], not
+    decreasing) are the last tokens of request r, already in the cache; without
+    ``starts`` every request has one (T = R).  The token at position p sees
+    the keys lo <= j < hi of its request's n tokens:
+
+      lo = max(0, p - window + 1, first[t])   window 0: none; first int32 [T]
+      hi = max(p + 1, min(prefix[r], n))      prefix int32 [R]
+
+    that is causal attention, with ``window`` over the nearest keys, with
+    ``prefix`` tokens that see each other both ways, with ``first`` the start of the
+    token's document.  Scores are scale q.k (scale 1 / sqrt(D) by default),
+    capped to softcap * tanh(. / softcap) when ``softcap`` > 0, less
+    slopes[h] * |p - j| with ``slopes`` (float32 [Hq]).  A token that sees no
+    key gets zeros; what it does not see does not reach it, whatever the
+    cache holds there.
+
+    Returns [T, Hq, D] in q's type, the type its next reader multiplies in.  Rows
+    that belong to no request (padding) come back zero, or with ``out`` are left
+    as they were.  Tokens of q may lie apart, heads and dims must not.  All lengths
+    stay on the device, so a captured graph follows them."""
+    dev, qs, t, hq, d, scale, softcap, window, res = _dense_args(
+        q, kv, scale, softcap, slopes, window, first, out)
+    r = kv.requests
+    if starts is not None:
+        _check_ints("starts", starts, r + 1, dev)
+    elif t != r:
+        raise ValueError("expected one query token per request, or starts")
+    if prefix is not None:
+        _check_ints("prefix", prefix, r, dev)
+    if t == 0:
+        return res
+    ws = _lib.workspace(_lib.size("stk_paged_attention_workspace_bytes", t, r, hq, kv.hkv,
+                                  kv.width, kv.block, d, starts is not None), dev)
+    _device_call(dev, "stk_paged_attention", _lib.ptr(q), qs, _lib.dtype_code(q), t, r, hq,
+                 kv.hkv, kv.width, kv.block, d, kv.pages, _lib.ptr(kv.k_pages),
+                 _lib.ptr(kv.v_pages), _lib.ptr(kv.block_table), _lib.ptr(kv.nblocks),
+                 _lib.ptr(kv.ntokens), _lib.ptr(starts), scale, softcap, _lib.ptr(slopes),
+                 window, _lib.ptr(prefix), _lib.ptr(first), _lib.ptr(res), int(out is None),
+                 _lib.ptr(ws), ws.numel())
+    return res
+
+
+def shared_attention(q, kv, groups, shared, scale=None, softcap=0.0, slopes=None, window=0,
+                     first=None, out=None):
+    """``attention`` of one token per request where requests share leading blocks.
+
+    q [R, Hq, D].  Requests groups[i] .. groups[i + 1] - 1 (groups int32
+    [G + 1], not decreasing) hold the same pages in the first shared[i] (int32 [G])
+    blocks of their table rows, as requests over one system prompt do; a
+    shared block is full.  Those keys and values are read once for the whole group
+    and multiplied with all its queries together, the rest per request, and the
+    two parts joined.  Requests outside every group share nothing.  The other
+    arguments and the result are those of ``attention``."""
+    dev, qs, t, hq, d, scale, softcap, window, res = _dense_args(
+        q, kv, scale, softcap, slopes, window, first, out)
+    r = kv.requests
+    if t != r:
+        raise ValueError("expected one query token per request")
+    if groups.ndim != 1 or not 2 <= groups.shape[0] <= r + 1:
+        raise ValueError("expected int32 groups[G+1], 1 <= G <= R")
+    n = groups.shape[0] - 1
+    _check_ints("groups", groups, n + 1, dev)
+    _check_ints("shared", shared, n, dev)
+    ws = _lib.workspace(_lib.size("stk_paged_shared_workspace_bytes", r, n, hq, kv.hkv,
+                                  kv.width, kv.block, d), dev)
+    _device_call(dev, "stk_paged_shared_attention", _lib.ptr(q), qs, _lib.dtype_code(q), r, hq,
+                 kv.hkv, kv.width, kv.block, d, kv.pages, _lib.ptr(kv.k_pages),
+                 _lib.ptr(kv.v_pages), _lib.ptr(kv.block_table), _lib.ptr(kv.nblocks),
+                 _lib.ptr(kv.ntokens), _lib.ptr(groups), _lib.ptr(shared), n, scale, softcap,
+                 _lib.ptr(slopes), window, _lib.ptr(first), _lib.ptr(res), _lib.ptr(ws),
+                 ws.numel())
+    return res
+
+
 def _check(q, kv, predicted, topk):
     if not isinstance(kv, PagedKV):
         raise TypeError("kv must be a PagedKV")

@@ -3,9 +3,9 @@
 //
 // A tile is up to 128 query rows (token, head) of one KV head, so that the
 // heads of a KV group share its keys; four waves own 32 rows each, and walk
-// the tile's keys in units of TK.  K and V of a unit pass through LDS, double
-// buffered: the next unit's rows travel to registers while this one is
-// worked on, and one barrier per unit hands them over.
+// the tile's keys in units of TK.  K and V of a unit come straight into LDS
+// (no registers on the way), double buffered: the next unit travels while
+// this one is worked on, and one barrier per unit hands it over.
 //   S[key, row] = K Q^T (32x32x16), O^T[dim, row] += V^T P^T
 // Column `row` of both products is one lane (and its partner 32 lanes on), so
 // the softmax needs no exchange but that of the two halves' maxima, and the
@@ -16,10 +16,10 @@
 // neither read has bank conflicts.
 //
 // Masks are one range of keys per row; units that every row of the tile sees whole
-// (all but the first and last ones) skip them.  In the others a value that no
-// row sees is zeroed on its way to LDS, and should a value that some rows see
-// and others do not be infinite or NaN, the unit's product is done by rows,
-// skipping the hidden keys.
+// (all but the first and last ones) skip them.  In the others the values that no
+// row sees are zeroed in LDS; should a value that some rows see and others do
+// not be infinite or NaN (0 times which is not 0), the tile is done row by row
+// instead, each row reading the keys that it sees (slow_rows).
 #pragma once
 
 #include "dense.hpp"
@@ -31,6 +31,82 @@ __device__ __forceinline__ bool nonfinite16(u16x8 v, uint16_t expo) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) bad |= (v[i] & expo) == expo;
   return bad;
+}
+
+// 16 bytes per lane from base + off to LDS, lane after lane from byte `lds`
+// (wave-uniform) on.  Counted by vmcnt like any load; the compiler does not
+// know of the write, so the caller waits (copies_done) and passes a barrier
+// before it reads.  (Its own intrinsic makes the compiler wait for all of these
+// before every LDS read.)
+__device__ __forceinline__ void copy_to_lds(uint32_t lds, const uint16_t* base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds), "v"(off), "s"(base)
+               : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+
+// Up to 32 query rows from rown on against the keys [kbase, kend), one row after the
+// other: a lane is a key for the scores and D / 64 dims for the output, and
+// hidden keys and their values are not read.
+template <typename T, int D, int MODE>
+__device__ void slow_rows(const DenseArgs& a, int seq, int s0, int s1, int64_t rown, int kvh,
+                          const int32_t* row, int kbase, int kend, const Parts& to, int64_t pr) {
+  constexpr int E = D / STK_WAVE;
+  const int lane = lane_id();
+  for (int i = 0; i < 32; ++i, ++rown, ++pr) {
+    if (rown >= (int64_t)(s1 - s0) * a.g) return;
+    const int tok = s0 + (int)(rown / a.g), head = kvh * a.g + (int)(rown % a.g);
+    int p;
+    const Span sp = seq_span(a, seq, s0, s1, tok, p);
+    const uint16_t* q = a.q + (int64_t)tok * a.qs + (int64_t)head * D;
+    float slope = 0.f;
+    if constexpr (MODE & 2) slope = a.slopes[head] * 1.44269504f;
+    float m = -INFINITY, l = 0.f, o[E] = {};
+    const int lo = max(kbase, sp.lo), hi = min(kend, sp.hi);
+    for (int k0 = lo & ~15; k0 < hi; k0 += STK_WAVE) {
+      const int key = k0 + lane;
+      const int run = pool_row(a, row, min(key, hi - 1) & ~15);
+      const bool ok = key >= lo && key < hi && run >= 0;
+      const int64_t at = ((int64_t)max(run, 0) + (key & 15)) * D;
+      float s = 0.f;
+      if (ok)
+        for (int x = 0; x < D; ++x) s += cvt(T{q[x]}) * cvt(T{a.kp[at + x]});
+      s = ok ? score2<MODE>(a, s, slope, (float)(p - key)) : -INFINITY;
+      const float mx = fmaxf(m, wave_max(s)), ms = mx == -INFINITY ? 0.f : mx;
+      const float f = part_weight(m, mx), e = ok ? __builtin_amdgcn_exp2f(s - ms) : 0.f;
+      m = mx;
+      l = l * f + wave_sum(e);
+#pragma unroll
+      for (int x = 0; x < E; ++x) o[x] *= f;
+      const uint64_t seen = __ballot(ok);
+      for (int k = 0; k < STK_WAVE; ++k) {
+        if (!(seen >> k & 1)) continue;
+        const float ek = __builtin_bit_cast(
+            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, e), k));
+        const int rk = __builtin_amdgcn_readlane(run, k) + ((k0 + k) & 15);
+#pragma unroll
+        for (int x = 0; x < E; ++x)
+          o[x] += ek * cvt(T{a.vp[(int64_t)rk * D + lane + STK_WAVE * x]});
+      }
+    }
+    if (to.m) {
+#pragma unroll
+      for (int x = 0; x < E; ++x) to.o[pr * D + lane + STK_WAVE * x] = o[x];
+      if (lane == 0) {
+        to.m[pr] = m;
+        to.l[pr] = l;
+      }
+    } else {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int x = 0; x < E; ++x)
+        a.out[((int64_t)tok * a.hq + head) * D + lane + STK_WAVE * x] = to16<T>(o[x] * inv);
+    }
+  }
 }
 
 template <typename T, int D, int MODE>
@@ -45,10 +121,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
   constexpr int RP = 256 / CPR;         // rows per load instruction of the workgroup
   constexpr int KN = TK / RP;           // load instructions per unit and thread
   constexpr int GR = TK / 16;           // runs of 16 keys per unit
-  constexpr int PS = D == 64 ? 4 * 32 * TK : 8;   // room for P by rows beside K's own
   constexpr uint16_t EXPO = __is_same(T, bf16s) ? 0x7f80 : 0x7c00;
-  __shared__ __attribute__((aligned(16))) uint16_t s_k[2][TK * D], s_v[2][TK * D], s_p[PS];
-  __shared__ int s_bad[2];
+  __shared__ __attribute__((aligned(16))) uint16_t s_k[2][TK * D], s_v[2][TK * D];
+  __shared__ int s_bad;
   const int tid = threadIdx.x, lane = lane_id();
   const int w = __builtin_amdgcn_readfirstlane(wave_id());
   const int n32 = lane & 31, h = lane >> 5, i16 = lane & 15, gq = (lane >> 4) & 1;
@@ -91,20 +166,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
     }
     it = __builtin_amdgcn_readfirstlane(lo);
   }
-  if (tid < 2) s_bad[tid] = 0;
-  int serial = 0;                       // units handed over so far, in this workgroup
+  if (tid == 0) s_bad = 0;
+  int serial = 0;                       // units worked on so far, in this workgroup
 
   // LDS addresses (elements)
   auto fk = [](int row) { return D == 64 ? (row >> 1) & 7 : row & 15; };
   auto fv = [](int row) { return D == 64 ? (row >> 1) & 1 : row & 3; };
   const int lrow = tid / CPR, lch = tid % CPR;
-  int kw[KN], vw[KN], ka[KS], va[DB];
+  // byte offsets of this lane's K (for D = 256 of both halves of a run) and V chunk
+  uint32_t ko[2], vo;
 #pragma unroll
-  for (int i = 0; i < KN; ++i) {
-    const int row = i * RP + lrow;
-    kw[i] = row * D + (lch ^ fk(row)) * 8;
-    vw[i] = row * D + ((((lch >> 2) ^ fv(row)) << 2) | (lch & 3)) * 8;
-  }
+  for (int i = 0; i < 2; ++i)
+    ko[i] = ((lrow & 15) * D + (lch ^ fk(lrow + (D == 256 ? 8 * i : 0))) * 8) * 2;
+  vo = ((lrow & 15) * D + ((((lch >> 2) ^ fv(lrow)) << 2) | (lch & 3)) * 8) * 2;
+  int ka[KS], va[DB];
 #pragma unroll
   for (int s = 0; s < KS; ++s) ka[s] = n32 * D + ((2 * s + h) ^ fk(n32)) * 8;
 #pragma unroll
@@ -168,55 +243,48 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
       return key < kend ? x : -1;
     };
     int ent = window(0), nxt = window(1);
-    u16x8 kf[KN], vf[KN];
-    int rows[GR];                                     // of the unit in kf, vf
-    auto load = [&](int j) {
+    int vmask = 0;                                    // runs with a page, of the unit last issued
+    // Lane l of wave w fills the 16-byte slot 256 i + 64 w + l of the unit's LDS: row
+    // i RP + lrow, and of that row the chunk that the swizzle puts there.  A
+    // wave's rows lie in one run of 16 keys.
+    auto issue = [&](int j, int buf) {
       if (j > 0 && (j * GR) % 64 == 0) {
         ent = nxt;
         nxt = window(j * GR / 64 + 1);
       }
+      int rows[GR];
+      vmask = 0;
 #pragma unroll
-      for (int x = 0; x < GR; ++x) rows[x] = __builtin_amdgcn_readlane(ent, (j * GR + x) & 63);
-#pragma unroll
-      for (int i = 0; i < KN; ++i) {
-        // this wave's rows of load i lie in one run of 16 keys
-        const int run = (i * RP + w * (RP / 4)) / 16;
-        const int x = D == 64 ? (w < 2 ? rows[2 * i < GR ? 2 * i : 0] : rows[2 * i + 1 < GR ? 2 * i + 1 : 0])
-                              : rows[i * RP / 16];
-        const int64_t at = (int64_t)max(x, 0) * D;
-        const int off = (i * RP + lrow - 16 * run) * D + 8 * lch;
-        kf[i] = *reinterpret_cast<const u16x8*>(a.kp + at + off);
-        vf[i] = *reinterpret_cast<const u16x8*>(a.vp + at + off);
-      }
-    };
-    // unit j sees no mask
-    auto inner = [&](int key0) {
-      bool ok = key0 >= max_lo && key0 + TK <= min_hi;
-#pragma unroll
-      for (int x = 0; x < GR; ++x) ok = ok && rows[x] >= 0;
-      return ok;
-    };
-    int crow[GR];                                     // of the unit in LDS
-    auto stage = [&](int j, int buf) {                // kf, vf to LDS
-      const int key0 = kbase + j * TK;
-      if (!inner(key0)) {
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < KN; ++i) {
-          const int kr = i * RP + lrow, key = key0 + kr;
-          bool ok = key >= klo && key < khi;
-#pragma unroll
-          for (int x = 0; x < GR; ++x) ok = ok && !(kr / 16 == x && rows[x] < 0);
-          if (!ok) vf[i] = u16x8{};
-          bad |= nonfinite16(vf[i], EXPO);
-        }
-        if (bad) s_bad[buf] = serial + 1;
+      for (int x = 0; x < GR; ++x) {
+        rows[x] = __builtin_amdgcn_readlane(ent, (j * GR + x) & 63);
+        vmask |= rows[x] >= 0 ? 1 << x : 0;
       }
 #pragma unroll
       for (int i = 0; i < KN; ++i) {
-        *reinterpret_cast<u16x8*>(s_k[buf] + kw[i]) = kf[i];
-        *reinterpret_cast<u16x8*>(s_v[buf] + vw[i]) = vf[i];
+        int x = rows[D == 64 ? 2 * i : i * RP / 16];
+        if (D == 64 && w >= 2) x = rows[D == 64 ? 2 * i + 1 : 0];
+        const int64_t at = (int64_t)max(x, 0) * D + (i * RP % 16) * D;
+        const uint32_t slot = (uint32_t)(256 * i + 64 * w) * 16;
+        copy_to_lds(lds_address(s_k[buf]) + slot, a.kp + at, ko[i * RP % 16 ? 1 : 0]);
+        copy_to_lds(lds_address(s_v[buf]) + slot, a.vp + at, vo);
       }
+    };
+    // whether some row of the tile does not see all of the unit
+    auto masked = [&](int key0) {
+      return !(key0 >= max_lo && key0 + TK <= min_hi && vmask == (1 << GR) - 1);
+    };
+    // Values of the unit that no row sees become zero; s_bad = serial if any other
+    // is not finite.
+    auto clean = [&](int key0, int mask, uint16_t* lv) {
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < KN; ++i) {
+        const int kr = i * RP + lrow, key = key0 + kr;
+        u16x8* at = reinterpret_cast<u16x8*>(lv + (256 * i + tid) * 8);
+        if (key >= klo && key < khi && (mask >> (kr / 16) & 1)) bad |= nonfinite16(*at, EXPO);
+        else *at = u16x8{};
+      }
+      if (bad) s_bad = serial;
     };
 
     float m = -INFINITY, l = 0.f;
@@ -226,34 +294,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
 #pragma unroll
       for (int x = 0; x < 16; ++x) acc[i][x] = 0.f;
 
-    load(0);
-    __syncthreads();                                  // the last item's LDS reads are done
-    stage(0, 0);
-    bool edge = !inner(kbase);
+    // P of the unit whose K is lk, as the second product's operand; m, l and
+    // the output follow its maximum
+    auto weights = [&](const uint16_t* lk, int key0, bool edge, int mask,
+                       u16x8 (&pf)[TK / 16]) {
+      f32x16 s[KB];
 #pragma unroll
-    for (int x = 0; x < GR; ++x) crow[x] = rows[x];
-    if (cnt > 1) load(1);
-    for (int j = 0; j < cnt; ++j) {
-      const int buf = j & 1, key0 = kbase + j * TK;
-      __syncthreads();
-      ++serial;
-      const bool bad = edge && s_bad[buf] == serial;
-      const uint16_t* lk = s_k[buf];
-      const uint16_t* lv = s_v[buf];
-      const bool work = key0 < whi && key0 + TK > wlo;
-      u16x8 pf[TK / 16];
-      if (work) {
-        f32x16 s[KB];
+      for (int b = 0; b < KB; ++b) {
 #pragma unroll
-        for (int b = 0; b < KB; ++b) {
+        for (int x = 0; x < 16; ++x) s[b][x] = 0.f;
 #pragma unroll
-          for (int x = 0; x < 16; ++x) s[b][x] = 0.f;
-#pragma unroll
-          for (int x = 0; x < KS; ++x)
-            s[b] = mma32<T>(*reinterpret_cast<const u16x8*>(lk + ka[x] + 32 * b * D), qf[x], s[b]);
-        }
+        for (int x = 0; x < KS; ++x)
+          s[b] = mma32<T>(*reinterpret_cast<const u16x8*>(lk + ka[x] + 32 * b * D), qf[x], s[b]);
+      }
+      // MODE 0 keeps the products as they are: their scale goes into the exponent's FMA
+      const float sc = MODE ? 1.f : a.c;
+      if constexpr (MODE != 0) {
         const float dist = (float)(p - key0 - 4 * h);
-        float top = -INFINITY;
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
@@ -261,95 +318,85 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
             const int off = 32 * b + 8 * (x / 4) + x % 4;
             s[b][x] = score2<MODE>(a, s[b][x], slope, dist - (float)off);
           }
-        if (edge) {
-#pragma unroll
-          for (int b = 0; b < KB; ++b)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              const int key = key0 + 4 * h + 32 * b + 8 * (x / 4) + x % 4;
-              const bool ok = key >= sp.lo && key < sp.hi && crow[2 * b + x / 8] >= 0;
-              s[b][x] = ok ? s[b][x] : -INFINITY;
-            }
-        }
-#pragma unroll
-        for (int b = 0; b < KB; ++b)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) top = fmaxf(top, s[b][x]);
-        if (__any(top > m + kLazy)) {
-          float mx = fmaxf(top, m);
-          mx = fmaxf(mx, __shfl_xor(mx, 32));
-          const float f = mx == m ? 1.f : __builtin_amdgcn_exp2f(m - mx);
-          m = mx;
-          l *= f;
-#pragma unroll
-          for (int i = 0; i < DB; ++i) acc[i] *= f;
-        }
-        const float ms = m == -INFINITY ? 0.f : m;
+      }
+      if (edge) {
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
-            const float e = __builtin_amdgcn_exp2f(s[b][x] - ms);
-            l += e;
-            pf[2 * b + x / 8][x % 8] = to16<T>(e);
+            const int key = key0 + 4 * h + 32 * b + 8 * (x / 4) + x % 4;
+            const bool ok = key >= sp.lo && key < sp.hi && (mask >> (2 * b + x / 8) & 1);
+            s[b][x] = ok ? s[b][x] : -INFINITY;
           }
       }
-      if (!bad) {
-        if (work) {
+      float top = s[0][0];
 #pragma unroll
-          for (int x = 0; x < TK / 16; ++x)
+      for (int b = 0; b < KB; ++b)
 #pragma unroll
-            for (int db = 0; db < DB; ++db) {
-              const u16x4 lo = lds_tr(lv + va[db] + 16 * x * D);
-              const u16x4 hi = lds_tr(lv + va[db] + (16 * x + 8) * D);
-              acc[db] = mma32<T>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pf[x],
-                                 acc[db]);
-            }
+        for (int x = 0; x < 16; ++x) top = fmaxf(top, s[b][x]);
+      top *= sc;
+      if (__any(top > m + kLazy)) {
+        float mx = fmaxf(top, m);
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float f = mx == m ? 1.f : __builtin_amdgcn_exp2f(m - mx);
+        m = mx;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < DB; ++i) acc[i] *= f;
+      }
+      const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][x], sc, -ms));
+          l += e;
+          pf[2 * b + x / 8][x % 8] = to16<T>(e);
         }
-      } else {
-        // some value is infinite or NaN: by rows, hidden keys skipped.  P goes
-        // through the unit's K (all waves are past it) or, at D = 64, its own room.
+    };
+
+    __syncthreads();                                  // the last item's LDS reads are done
+    issue(0, 0);
+    bool bad = false;                                 // some rows must skip a value
+    for (int j = 0; j < cnt && !bad; ++j) {
+      const int buf = j & 1, key0 = kbase + j * TK;
+      const int mask = vmask;
+      const bool edge = masked(key0);
+      ++serial;
+      copies_done();
+      __syncthreads();
+      if (j + 1 < cnt) issue(j + 1, buf ^ 1);
+      if (edge) {
+        clean(key0, mask, s_v[buf]);
         __syncthreads();
-        if (work) {
-          uint16_t* sp16 = (D == 64 ? s_p : s_k[buf]) + w * 32 * TK;
-#pragma unroll
-          for (int x = 0; x < TK / 16; ++x)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              sp16[n32 * TK + 16 * x + 8 * (e / 4) + 4 * h + e % 4] = pf[x][e];
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-          for (int k = 0; k < TK; ++k) {
-            const float pk = cvt(T{sp16[n32 * TK + k]});
-            const int key = key0 + k;
-            const bool ok = key >= sp.lo && key < sp.hi;
-#pragma unroll
-            for (int db = 0; db < DB; ++db)
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                // dims 32 db + 8 x + 4 h .. + 3
-                const u16x4 v4 = *reinterpret_cast<const u16x4*>(
-                    lv + k * D + (db ^ fv(k)) * 32 + 8 * x + 4 * h);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float o = acc[db][4 * x + e];
-                  acc[db][4 * x + e] = ok ? o + pk * cvt(T{v4[e]}) : o;
-                }
-              }
-          }
-        }
+        bad = s_bad == serial;
       }
-      if (j + 1 < cnt) {
-        stage(j + 1, buf ^ 1);
-        edge = !inner(key0 + TK);
+      if (!bad && key0 < whi && key0 + TK > wlo) {
+        u16x8 pf[TK / 16];
+        weights(s_k[buf], key0, edge, mask, pf);
+        const uint16_t* lv = s_v[buf];
 #pragma unroll
-        for (int x = 0; x < GR; ++x) crow[x] = rows[x];
-        if (j + 2 < cnt) load(j + 2);
+        for (int x = 0; x < TK / 16; ++x)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            const u16x4 lo = lds_tr(lv + va[db] + 16 * x * D);
+            const u16x4 hi = lds_tr(lv + va[db] + (16 * x + 8) * D);
+            acc[db] = mma32<T>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pf[x],
+                               acc[db]);
+          }
       }
     }
-    l += __shfl_xor(l, 32);
     const bool all = j0 == 0 && j1 == n;
-    if (valid) {
+    if (bad) {
+      copies_done();
+      __syncthreads();
+      const int64_t slot = all ? (int64_t)kvh * ntiles + it
+                               : 2 * (int64_t)blockIdx.x + (j0 > 0 ? 0 : 1);
+      slow_rows<T, D, MODE>(a, seq, s0, s1, (int64_t)tile * kDenseRows + 32 * w, kvh, row, kbase,
+                            kend, all ? whole : split, slot * kDenseRows + 32 * w);
+    }
+    l += __shfl_xor(l, 32);
+    if (valid && !bad) {
       if (all && !whole.m) {
         uint16_t* o = a.out + ((int64_t)tok * a.hq + head) * D + 4 * h;
 #pragma unroll

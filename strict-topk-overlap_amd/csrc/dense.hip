@@ -79,28 +79,35 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(DenseArgs a, Plan pl, int
   }
 }
 
-// Rows of the tiles whose units were dealt to several workgroups.
+// Rows of the tiles whose units were dealt to several workgroups, kJoinRows of
+// them per workgroup.
+constexpr int kJoinRows = 16;
 template <typename T, int D>
-__global__ __launch_bounds__(256) void k_join_tiles(DenseArgs a, Plan pl, Parts split, int launched) {
+__global__ __launch_bounds__(256) void k_join_tiles(DenseArgs a, Plan pl, Parts split,
+                                                    int launched) {
+  constexpr int SL = kDenseRows / kJoinRows;
   const int per = pl.head[0], ntiles = pl.head[1];
-  const int kvh = (int)blockIdx.x / pl.limit, it = (int)blockIdx.x % pl.limit;
+  const int kvh = (int)blockIdx.x / (pl.limit * SL), x0 = (int)blockIdx.x % (pl.limit * SL);
+  const int it = x0 / SL, r0 = (x0 % SL) * kJoinRows;
   if (it >= ntiles) return;
   const Tile t = pl.tiles[it];
-  const int64_t total = (int64_t)per * a.hkv, first = (int64_t)kvh * per + t.cum;
+  const int first = kvh * per + t.cum;
   const int n = (it + 1 < ntiles ? pl.tiles[it + 1].cum : per) - t.cum;
-  const int grid = split_grid(total, launched);
-  const int w0 = wg_of(total, first, grid), w1 = wg_of(total, first + n - 1, grid);
+  const Deal deal(per * a.hkv, launched);
+  const int w0 = deal.wg_of(first), w1 = deal.wg_of(first + n - 1);
   if (w0 == w1) return;
   int s0, s1;
   seq_rows(a, t.seq, s0, s1);
-  const int64_t row0 = (int64_t)t.tile * kDenseRows;
-  const int nrow = (int)min((int64_t)kDenseRows, (int64_t)(s1 - s0) * a.g - row0);
+  const int64_t row0 = (int64_t)t.tile * kDenseRows + r0;
+  const int nrow = (int)min((int64_t)kJoinRows, (int64_t)(s1 - s0) * a.g - row0);
+#pragma unroll 2
   for (int x = threadIdx.x; x < nrow * (D / 4); x += 256) {
     const int row = x / (D / 4), dc = x % (D / 4);
     float m = -INFINITY, l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int w = w0; w <= w1; ++w) {
-      const int64_t pr = (2 * (int64_t)w + (w == w0 ? 1 : 0)) * kDenseRows + row;
+      const int64_t pr = (2 * (int64_t)w + (w == w0 ? 1 : 0)) * kDenseRows + r0 + row;
       const float mi = split.m[pr], li = split.l[pr], mx = fmaxf(m, mi);
       const f32x4 oi = *reinterpret_cast<const f32x4*>(split.o + pr * D + 4 * dc);
       const float f = part_weight(m, mx), fi = part_weight(mi, mx);
@@ -117,18 +124,19 @@ __global__ __launch_bounds__(256) void k_join_tiles(DenseArgs a, Plan pl, Parts 
 // with groups those of the shared keys.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Parts whole,
-                                                   int launched, Plan pl, Parts psplit,
-                                                   Parts pwhole, int plaunched) {
+                                                   const int32_t* place, int launched, Plan pl,
+                                                   Parts psplit, Parts pwhole, int plaunched) {
   constexpr int CH = D / 4, NP = 256 / CH;       // 4-wide columns, parts in flight
   __shared__ float s_m[NP], s_l[NP];
   __shared__ f32x4 s_o[NP][CH];
   const int r = (int)blockIdx.x / a.hq, head = (int)blockIdx.x % a.hq;
   const int kvh = head / a.g, gi = head % a.g, nc = decode_chunks(a);
   const int item = kvh * nc + gi / kDecodeRows, hrow = gi % kDecodeRows;
-  const DecodePlace at = decode_place<true>(a, r, 0);
-  const DecodeSpan sp = decode_span(a, r);
-  const int first = at.base + item * sp.n, grid = split_grid(at.total, launched);
-  const int w0 = wg_of(at.total, first, grid), w1 = wg_of(at.total, first + sp.n - 1, grid);
+  // a request's span is one unit or more for each of its items
+  const int base = place[r], total = place[a.requests];
+  const int n = (place[r + 1] - base) / (a.hkv * nc), first = base + item * n;
+  const Deal deal(total, launched);
+  const int w0 = deal.wg_of(first), w1 = deal.wg_of(first + n - 1);
   const int ns = w1 - w0 + 1;
   int np = 0, v0 = 0, rr = 0;
   int64_t pslot = 0;
@@ -142,11 +150,10 @@ __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Par
       rr = (int)(idx % kDenseRows);
       const int per = pl.head[0], ntiles = pl.head[1];
       const int cum = pl.tiles[it].cum;
-      const int n = (it + 1 < ntiles ? pl.tiles[it + 1].cum : per) - cum;
-      const int64_t total = (int64_t)per * a.hkv, pf = (int64_t)kvh * per + cum;
-      const int pgrid = split_grid(total, plaunched);
-      v0 = wg_of(total, pf, pgrid);
-      np = wg_of(total, pf + n - 1, pgrid) - v0 + 1;
+      const int pn = (it + 1 < ntiles ? pl.tiles[it + 1].cum : per) - cum;
+      const Deal pdeal(per * a.hkv, plaunched);
+      v0 = pdeal.wg_of(kvh * per + cum);
+      np = pdeal.wg_of(kvh * per + cum + pn - 1) - v0 + 1;
       pslot = (int64_t)kvh * ntiles + it;
     }
   } else if (ns == 1) {
@@ -155,6 +162,7 @@ __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Par
   const int dc = threadIdx.x % CH, grp = threadIdx.x / CH;
   float m = -INFINITY, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int i = grp; i < ns + np; i += NP) {
     const float *pm, *pl_, *po;
     int64_t pr;
@@ -235,10 +243,14 @@ static int64_t prefill_units(const DenseShape& s) {
   const int tk = s.d == 256 ? 32 : 64;
   return tile_limit(s) * s.hkv * (((int64_t)s.nb * s.b + tk - 1) / tk + 1);
 }
-// Tiles that fill the device several times over need no splitting.
-constexpr int64_t kDirectTiles = 4 * kFill;
+// Tiles that fill the device several times over need no splitting, and neither do
+// those of caches that hold few units: without it there is nothing to list and
+// nothing to join.
+constexpr int64_t kDirectTiles = 4 * kFill, kDirectUnits = 8;
 static bool prefill_direct(const DenseShape& s) {
-  return !s.ngroups && tile_limit(s) * s.hkv >= kDirectTiles;
+  const int tk = s.d == 256 ? 32 : 64;
+  return !s.ngroups && (tile_limit(s) * s.hkv >= kDirectTiles ||
+                        (int64_t)s.nb * s.b <= kDirectUnits * tk);
 }
 static int prefill_grid(const DenseShape& s) {
   if (prefill_direct(s)) return (int)(tile_limit(s) * s.hkv);
@@ -277,15 +289,16 @@ static size_t dense_bytes(const DenseShape& s) {
   const int nc = (s.hq / s.hkv + kDecodeRows - 1) / kDecodeRows;
   size_t x = 0;
   if (!s.ragged) {
-    x += parts_bytes(2 * (int64_t)decode_grid(s), kDecodeRows, s.d);
+    x += stk_align((s.requests + 1) * sizeof(int32_t)) +
+         parts_bytes(2 * (int64_t)decode_grid(s), kDecodeRows, s.d);
     if (s.ngroups) x += parts_bytes((int64_t)s.requests * s.hkv * nc, kDecodeRows, s.d);
   }
   if (s.ragged || s.ngroups) {
-    x += plan_bytes(s);
-    if (!prefill_direct(s)) x += parts_bytes(2 * (int64_t)prefill_grid(s), kDenseRows, s.d);
+    if (!prefill_direct(s))
+      x += plan_bytes(s) + parts_bytes(2 * (int64_t)prefill_grid(s), kDenseRows, s.d);
     if (s.ngroups) x += parts_bytes(tile_limit(s) * s.hkv, kDenseRows, s.d);
   }
-  return x;
+  return x ? x : 256;
 }
 
 static int launch_plan(const DenseArgs& a, const Plan& p, int d, hipStream_t st) {
@@ -296,7 +309,7 @@ static int launch_plan(const DenseArgs& a, const Plan& p, int d, hipStream_t st)
 template <typename T>
 static void launch_join_tiles(const DenseArgs& a, const Plan& p, const Parts& split, int grid,
                               int d, hipStream_t st) {
-  const dim3 g((unsigned)(p.limit * a.hkv));
+  const dim3 g((unsigned)(p.limit * a.hkv * (kDenseRows / kJoinRows)));
   if (d == 64) hipLaunchKernelGGL((k_join_tiles<T, 64>), g, dim3(256), 0, st, a, p, split, grid);
   else if (d == 128)
     hipLaunchKernelGGL((k_join_tiles<T, 128>), g, dim3(256), 0, st, a, p, split, grid);
@@ -304,12 +317,13 @@ static void launch_join_tiles(const DenseArgs& a, const Plan& p, const Parts& sp
 }
 
 template <typename T>
-static void launch_join_rows(const DenseArgs& a, const Parts& split, const Parts& whole, int grid,
-                             const Plan& p, const Parts& ps, const Parts& pw, int pgrid, int d,
+static void launch_join_rows(const DenseArgs& a, const Parts& split, const Parts& whole,
+                             const int32_t* place, int grid, const Plan& p, const Parts& ps, const Parts& pw, int pgrid, int d,
                              hipStream_t st) {
   const dim3 g((unsigned)(a.requests * a.hq));
 #define STK_JOIN(D) \
-  hipLaunchKernelGGL((k_join_rows<T, D>), g, dim3(256), 0, st, a, split, whole, grid, p, ps, pw, pgrid)
+  hipLaunchKernelGGL((k_join_rows<T, D>), g, dim3(256), 0, st, a, split, whole, place, \
+                     grid, p, ps, pw, pgrid)
   if (d == 64) STK_JOIN(64);
   else if (d == 128) STK_JOIN(128);
   else STK_JOIN(256);
@@ -321,19 +335,21 @@ static int run_dense(const DenseShape& s, DenseArgs a, int mode, void* workspace
   Carve c(workspace);
   const Parts none{nullptr, nullptr, nullptr};
   if (s.ragged) {
-    const Plan p = take_plan(c, s);
-    const bool direct = prefill_direct(s);
     const int grid = prefill_grid(s);
-    const Parts split = direct ? none : take_parts(c, 2 * (int64_t)grid, kDenseRows, s.d);
+    if (prefill_direct(s))
+      return launch_prefill<T>(s.d, mode, a, Plan{}, none, none, grid, true, st);
+    const Plan p = take_plan(c, s);
+    const Parts split = take_parts(c, 2 * (int64_t)grid, kDenseRows, s.d);
     int rc = launch_plan(a, p, s.d, st);
     if (rc) return rc;
-    rc = launch_prefill<T>(s.d, mode, a, p, split, none, grid, direct, st);
-    if (rc || direct) return rc;
+    rc = launch_prefill<T>(s.d, mode, a, p, split, none, grid, false, st);
+    if (rc) return rc;
     launch_join_tiles<T>(a, p, split, grid, s.d, st);
     return stk_check_launch("k_join_tiles");
   }
   const int nc = (a.g + kDecodeRows - 1) / kDecodeRows;
   const int grid = decode_grid(s);
+  int32_t* place = c.take<int32_t>(s.requests + 1);
   const Parts split = take_parts(c, 2 * (int64_t)grid, kDecodeRows, s.d);
   Parts whole = none, ps = none, pw = none;
   Plan p{};
@@ -349,9 +365,9 @@ static int run_dense(const DenseShape& s, DenseArgs a, int mode, void* workspace
     rc = launch_prefill<T>(s.d, mode, a, p, ps, pw, pgrid, false, st);
     if (rc) return rc;
   }
-  int rc = launch_decode<T>(s.d, mode, a, split, whole, grid, st);
+  int rc = launch_decode<T>(s.d, mode, a, split, whole, place, grid, st);
   if (rc) return rc;
-  launch_join_rows<T>(a, split, whole, grid, p, ps, pw, pgrid, s.d, st);
+  launch_join_rows<T>(a, split, whole, place, grid, p, ps, pw, pgrid, s.d, st);
   return stk_check_launch("k_join_rows");
 }
 

@@ -177,21 +177,22 @@ __device__ __forceinline__ void store_out(uint16_t* p, f32x4 o, float sum) {
   *reinterpret_cast<u16x4*>(p) = y;
 }
 
-// Work of a split grid: `total` units dealt evenly to the first `grid`
-// workgroups (at most one per unit, so that none of them is without work),
-// workgroup w taking [unit_at(w), unit_at(w + 1)).
-__device__ __forceinline__ int split_grid(int64_t total, int launched) {
-  return (int)min(total, (int64_t)launched);
-}
-__device__ __forceinline__ int64_t unit_at(int64_t total, int w, int grid) {
-  return total * w / grid;
-}
-// The workgroup that holds unit u.
-__device__ __forceinline__ int wg_of(int64_t total, int64_t u, int grid) {
-  int w = (int)(u * grid / total);
-  while (w + 1 < grid && unit_at(total, w + 1, grid) <= u) ++w;
-  return w;
-}
+// Work of a split grid: `total` units dealt evenly to its first workgroups (at
+// most one per unit, so that none of them is without work), workgroup w taking
+// [at(w), at(w + 1)).
+struct Deal {
+  uint32_t grid, q, rem;
+  __device__ __forceinline__ Deal(int total, int launched) {
+    grid = (uint32_t)min(total, launched);
+    q = (uint32_t)total / grid;
+    rem = (uint32_t)total - q * grid;
+  }
+  __device__ __forceinline__ int at(int w) const { return (int)(w * q + min((uint32_t)w, rem)); }
+  __device__ __forceinline__ int wg_of(int u) const {      // the workgroup that holds unit u
+    const uint32_t big = rem * (q + 1);
+    return (int)((uint32_t)u < big ? (uint32_t)u / (q + 1) : rem + ((uint32_t)u - big) / q);
+  }
+};
 
 // Row tiles of the attention of many rows (dense_prefill.hpp), listed on the
 // device: tile `tile` of sequence `seq` reads units of keys from kstart on,
@@ -237,7 +238,7 @@ __device__ __forceinline__ Span seq_span(const DenseArgs& a, int q, int s0, int 
 // dense_decode_*.hip, dense_prefill_*.hip: one element type each
 template <typename T>
 int launch_decode(int d, int mode, const DenseArgs& a, const Parts& split, const Parts& whole,
-                  int grid, hipStream_t st);
+                  int32_t* place, int grid, hipStream_t st);
 template <typename T>
 int launch_prefill(int d, int mode, const DenseArgs& a, const Plan& p, const Parts& split,
                    const Parts& whole, int grid, bool direct, hipStream_t st);

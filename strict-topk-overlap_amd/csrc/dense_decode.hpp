@@ -5,7 +5,7 @@
 // are dealt evenly over one grid that fills the device: a ragged batch, or one long
 // request, keeps every CU busy to the end.  A workgroup walks its run of units
 // item by item.  Items that lie whole in one workgroup are finished there; the
-// parts of the others are joined by k_join.  Nothing of this needs the lengths on
+// parts of the others are joined by k_join_rows.  Nothing of this needs the lengths on
 // the host.
 //
 // Within a workgroup the four waves take a quarter of the keys each and share
@@ -45,13 +45,14 @@ __device__ __forceinline__ int decode_chunks(const DenseArgs& a) {
   return (a.g + kDecodeRows - 1) / kDecodeRows;
 }
 
-// The requests' units laid end to end: how many there are, a request, and the
-// units before it.  BY_REQUEST: request `want`; else the request that holds
-// the first unit of workgroup `want` (past the last one with work: any).
+// The requests' units laid end to end: how many there are, the request that holds
+// the first unit of workgroup `wg` of `launched`, and the units before that
+// request (past the last workgroup with work: any).  Workgroup 0 also leaves
+// the units before every request, and their total, in place [R + 1] for k_join_rows.
 struct DecodePlace { int total, base, r; };
 
-template <bool BY_REQUEST>
-__device__ __forceinline__ DecodePlace decode_place(const DenseArgs& a, int want, int launched) {
+__device__ __forceinline__ DecodePlace decode_place(const DenseArgs& a, int wg, int launched,
+                                                    int32_t* place) {
   __shared__ int s_tmp[4], s_at[2];
   const int per = a.hkv * decode_chunks(a);
   int total = 0, c0 = 0, b0 = 0, sum0 = 0;
@@ -61,7 +62,7 @@ __device__ __forceinline__ DecodePlace decode_place(const DenseArgs& a, int want
     int sum;
     __syncthreads();
     const int before = total + block_excl_scan1(c, s_tmp, &sum);
-    if (BY_REQUEST && r == want) s_at[0] = before;
+    if (wg == 0 && r < a.requests) place[r] = before;
     if (r0 == 0) {
       c0 = c;
       b0 = before;
@@ -69,33 +70,33 @@ __device__ __forceinline__ DecodePlace decode_place(const DenseArgs& a, int want
     }
     total += sum;
   }
-  if (!BY_REQUEST) {
-    const int u = (int)unit_at(total, want, split_grid(total, launched));
-    int base = 0;
-    for (int r0 = 0; r0 < a.requests; r0 += 256) {
-      const int r = r0 + (int)threadIdx.x;
-      int c = c0, before = b0, sum = sum0;
-      if (r0 > 0) {
-        c = r < a.requests ? decode_span(a, r).n * per : 0;
-        __syncthreads();
-        before = base + block_excl_scan1(c, s_tmp, &sum);
-      }
-      if (u >= before && u < before + c) {
-        s_at[0] = before;
-        s_at[1] = r;
-      }
-      base += sum;
+  if (wg == 0 && threadIdx.x == 0) place[a.requests] = total;
+  const int u = Deal(total, launched).at(wg);
+  int base = 0;
+  for (int r0 = 0; r0 < a.requests; r0 += 256) {
+    const int r = r0 + (int)threadIdx.x;
+    int c = c0, before = b0, sum = sum0;
+    if (r0 > 0) {
+      c = r < a.requests ? decode_span(a, r).n * per : 0;
+      __syncthreads();
+      before = base + block_excl_scan1(c, s_tmp, &sum);
     }
+    if (u >= before && u < before + c) {
+      s_at[0] = before;
+      s_at[1] = r;
+    }
+    base += sum;
   }
   __syncthreads();
-  DecodePlace p{total, s_at[0], BY_REQUEST ? want : s_at[1]};
+  DecodePlace p{total, s_at[0], s_at[1]};
   p.base = __builtin_amdgcn_readfirstlane(p.base);
   p.r = __builtin_amdgcn_readfirstlane(p.r);
   return p;
 }
 
 template <typename T, int D, int MODE>
-__global__ __launch_bounds__(256, 2) void k_decode(DenseArgs a, Parts split, Parts whole) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_decode(DenseArgs a, Parts split, Parts whole,
+                                                   int32_t* place) {
   constexpr int KS = D / 32;            // QK steps
   constexpr int DB = D / 16;            // output blocks
   constexpr int VN = D / 16;            // 16-byte chunks of a V tile per lane
@@ -106,11 +107,11 @@ __global__ __launch_bounds__(256, 2) void k_decode(DenseArgs a, Parts split, Par
   const int lane = lane_id(), w = wave_id();
   const int n16 = lane & 15, kg = lane >> 4;
   const int nc = decode_chunks(a);
-  const DecodePlace at = decode_place<false>(a, (int)blockIdx.x, (int)gridDim.x);
-  const int grid = split_grid(at.total, (int)gridDim.x);
-  if ((int)blockIdx.x >= grid) return;
-  int u = (int)unit_at(at.total, (int)blockIdx.x, grid);
-  const int u1 = (int)unit_at(at.total, (int)blockIdx.x + 1, grid);
+  const DecodePlace at = decode_place(a, (int)blockIdx.x, (int)gridDim.x, place);
+  const Deal deal(at.total, (int)gridDim.x);
+  if (blockIdx.x >= deal.grid) return;
+  int u = deal.at((int)blockIdx.x);
+  const int u1 = deal.at((int)blockIdx.x + 1);
   int r = at.r, base = at.base;
   // V tile in LDS: row-major, 32-byte blocks swizzled so that the 16 rows of a
   // transposed read spread over all banks

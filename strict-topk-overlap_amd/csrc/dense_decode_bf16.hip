@@ -5,17 +5,17 @@ namespace stk {
 
 template <>
 int launch_decode<bf16s>(int d, int mode, const DenseArgs& a, const Parts& split, const Parts& whole,
-                         int grid, hipStream_t st) {
+                         int32_t* place, int grid, hipStream_t st) {
 #define STK_MODE(D)                                                                            \
   switch (mode) {                                                                              \
     case 0: hipLaunchKernelGGL((k_decode<bf16s, D, 0>), dim3(grid), dim3(256), 0, st, a, split, \
-                               whole); break;                                                  \
+                               whole, place); break;                                           \
     case 1: hipLaunchKernelGGL((k_decode<bf16s, D, 1>), dim3(grid), dim3(256), 0, st, a, split, \
-                               whole); break;                                                  \
+                               whole, place); break;                                           \
     case 2: hipLaunchKernelGGL((k_decode<bf16s, D, 2>), dim3(grid), dim3(256), 0, st, a, split, \
-                               whole); break;                                                  \
+                               whole, place); break;                                           \
     default: hipLaunchKernelGGL((k_decode<bf16s, D, 3>), dim3(grid), dim3(256), 0, st, a,       \
-                                split, whole);                                                 \
+                                split, whole, place);                                          \
   }
   if (d == 64) {
     STK_MODE(64)

@@ -109,6 +109,54 @@ __device__ void slow_rows(const DenseArgs& a, int seq, int s0, int s1, int64_t r
   }
 }
 
+// The tile of workgroup wg where every tile has its own: tiles of one KV head after
+// the other, dealt to the XCDs in runs, and within a sequence the last rows,
+// which see the most keys, first.  kvh = Hkv: none.
+struct TilePlace { int seq, tile, kvh; };
+
+__device__ __forceinline__ TilePlace tile_place(const DenseArgs& a, int wg) {
+  __shared__ int s_tmp[4], s_at[2];
+  const int ns = sequences(a);
+  auto tiles = [&](int q) {
+    int s0 = 0, s1 = 0;
+    if (q < ns) seq_rows(a, q, s0, s1);
+    return (int)(((int64_t)(s1 - s0) * a.g + kDenseRows - 1) / kDenseRows);
+  };
+  int total = 0, c0 = 0, b0 = 0, sum0 = 0;
+  for (int q0 = 0; q0 < ns; q0 += 256) {
+    const int c = tiles(q0 + (int)threadIdx.x);
+    int sum;
+    __syncthreads();
+    const int before = block_excl_scan1(c, s_tmp, &sum);
+    if (q0 == 0) {
+      c0 = c;
+      b0 = before;
+      sum0 = sum;
+    }
+    total += sum;
+  }
+  const int64_t all = min((int64_t)total * a.hkv, (int64_t)gridDim.x);
+  if (wg >= all) return TilePlace{0, 0, a.hkv};
+  const int x = xcd_remap(wg, (int)all), kvh = x / total, it = x % total;
+  int base = 0;
+  for (int q0 = 0; q0 < ns; q0 += 256) {
+    int c = c0, before = b0, sum = sum0;
+    if (q0 > 0) {
+      c = tiles(q0 + (int)threadIdx.x);
+      __syncthreads();
+      before = base + block_excl_scan1(c, s_tmp, &sum);
+    }
+    if (it >= before && it < before + c) {
+      s_at[0] = q0 + (int)threadIdx.x;
+      s_at[1] = before + c - 1 - it;
+    }
+    base += sum;
+  }
+  __syncthreads();
+  return TilePlace{__builtin_amdgcn_readfirstlane(s_at[0]),
+                   __builtin_amdgcn_readfirstlane(s_at[1]), kvh};
+}
+
 template <typename T, int D, int MODE>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, Plan pl,
                                                                    Parts split, Parts whole,
@@ -123,7 +171,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
   constexpr int GR = TK / 16;           // runs of 16 keys per unit
   constexpr uint16_t EXPO = __is_same(T, bf16s) ? 0x7f80 : 0x7c00;
   __shared__ __attribute__((aligned(16))) uint16_t s_k[2][TK * D], s_v[2][TK * D];
-  __shared__ int s_bad;
+  __shared__ int s_bad, s_range[4][4];
   const int tid = threadIdx.x, lane = lane_id();
   const int w = __builtin_amdgcn_readfirstlane(wave_id());
   const int n32 = lane & 31, h = lane >> 5, i16 = lane & 15, gq = (lane >> 4) & 1;
@@ -139,25 +187,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
     }
   }
 
-  const int per = pl.head[0], ntiles = pl.head[1];
-  int64_t u, u1;
-  int kvh, it;
+  int u = 0, u1 = 1, kvh, it = 0, per = 0, ntiles = 0, dseq = 0, dtile = 0;
   if (direct) {
-    const int total = ntiles * a.hkv;
-    if ((int)blockIdx.x >= total) return;
-    const int x = xcd_remap((int)blockIdx.x, total);
-    kvh = x / ntiles;
-    it = x % ntiles;
-    u = 0;
-    u1 = 1;
+    const TilePlace at = tile_place(a, (int)blockIdx.x);
+    if (at.kvh >= a.hkv) return;
+    kvh = at.kvh;
+    dseq = at.seq;
+    dtile = at.tile;
   } else {
-    const int64_t total = (int64_t)per * a.hkv;
-    const int grid = split_grid(total, (int)gridDim.x);
-    if ((int)blockIdx.x >= grid) return;
-    u = unit_at(total, (int)blockIdx.x, grid);
-    u1 = unit_at(total, (int)blockIdx.x + 1, grid);
-    kvh = (int)(u / per);
-    const int rem = (int)(u % per);
+    per = pl.head[0];
+    ntiles = pl.head[1];
+    const Deal deal(per * a.hkv, (int)gridDim.x);
+    if (blockIdx.x >= deal.grid) return;
+    u = deal.at((int)blockIdx.x);
+    u1 = deal.at((int)blockIdx.x + 1);
+    kvh = u / per;
+    const int rem = u - kvh * per;
     int lo = 0, hi = ntiles - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
@@ -189,24 +234,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
   }
 
   while (u < u1) {
-    const Tile tl = pl.tiles[it];
+    Tile tl{dseq, dtile, 0, 0, 0, 0, 0, 0};
+    if (!direct) tl = pl.tiles[it];
     const int seq = __builtin_amdgcn_readfirstlane(tl.seq);
     const int tile = __builtin_amdgcn_readfirstlane(tl.tile);
-    const int kstart = __builtin_amdgcn_readfirstlane(tl.kstart);
-    const int klo = __builtin_amdgcn_readfirstlane(tl.klo);
-    const int khi = __builtin_amdgcn_readfirstlane(tl.khi);
-    const int max_lo = __builtin_amdgcn_readfirstlane(tl.max_lo);
-    const int min_hi = __builtin_amdgcn_readfirstlane(tl.min_hi);
-    const int n = max(1, (khi - kstart + TK - 1) / TK);
-    int j0 = 0, j1 = n;
-    if (!direct) {
-      const int64_t first = (int64_t)kvh * per + __builtin_amdgcn_readfirstlane(tl.cum);
-      j0 = (int)(u - first);
-      j1 = (int)min((int64_t)n, j0 + (u1 - u));
-      u += j1 - j0;
-    } else {
-      u = u1;
-    }
     int s0, s1;
     seq_rows(a, seq, s0, s1);
     const int64_t rown = (int64_t)tile * kDenseRows + 32 * w + n32;
@@ -215,10 +246,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
     const int head = kvh * a.g + (int)(valid ? rown % a.g : 0);
     int p = 0;
     Span sp = seq_span(a, seq, s0, s1, tok, p);
-    if (!valid) sp = Span{0, 0x7fffffff};
     // keys that some row of this wave sees
     int wlo = valid && sp.hi > sp.lo ? sp.lo : 0x7fffffff;
     int whi = valid && sp.hi > sp.lo ? sp.hi : 0;
+    int mlo = valid ? sp.lo : 0, mhi = valid ? (sp.hi > sp.lo ? sp.hi : 0) : 0x7fffffff;
+    if (!valid) sp = Span{0, 0x7fffffff};
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       wlo = min(wlo, __shfl_xor(wlo, o));
@@ -226,6 +258,39 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
     }
     wlo = __builtin_amdgcn_readfirstlane(wlo);
     whi = __builtin_amdgcn_readfirstlane(whi);
+    if (direct) {
+      // the tile's range from its rows, as k_plan lists it
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        mlo = max(mlo, __shfl_xor(mlo, o));
+        mhi = min(mhi, __shfl_xor(mhi, o));
+      }
+      if (lane == 0) {
+        s_range[w][0] = wlo;
+        s_range[w][1] = whi;
+        s_range[w][2] = mlo;
+        s_range[w][3] = mhi;
+      }
+      __syncthreads();
+      tl.klo = min(min(s_range[0][0], s_range[1][0]), min(s_range[2][0], s_range[3][0]));
+      tl.khi = max(max(s_range[0][1], s_range[1][1]), max(s_range[2][1], s_range[3][1]));
+      tl.max_lo = max(max(s_range[0][2], s_range[1][2]), max(s_range[2][2], s_range[3][2]));
+      tl.min_hi = min(min(s_range[0][3], s_range[1][3]), min(s_range[2][3], s_range[3][3]));
+      if (tl.khi <= tl.klo) tl.klo = tl.khi = 0;
+      tl.kstart = tl.klo & ~15;
+    }
+    const int kstart = __builtin_amdgcn_readfirstlane(tl.kstart);
+    const int klo = __builtin_amdgcn_readfirstlane(tl.klo);
+    const int khi = __builtin_amdgcn_readfirstlane(tl.khi);
+    const int max_lo = __builtin_amdgcn_readfirstlane(tl.max_lo);
+    const int min_hi = __builtin_amdgcn_readfirstlane(tl.min_hi);
+    const int n = max(1, (khi - kstart + TK - 1) / TK);
+    int j0 = 0, j1 = n;
+    if (!direct) {
+      j0 = u - (kvh * per + __builtin_amdgcn_readfirstlane(tl.cum));
+      j1 = min(n, j0 + (u1 - u));
+    }
+    u += direct ? 1 : j1 - j0;
     u16x8 qf[KS];
     const uint16_t* qp = a.q + (int64_t)tok * a.qs + (int64_t)head * D + 8 * h;
 #pragma unroll

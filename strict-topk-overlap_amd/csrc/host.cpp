@@ -1,6 +1,7 @@
 // Native host path of the fused steps' Python entry points: argument checks,
 // output allocation and the C-ABI call of step.speculative_step,
-// paged.speculative_step, paged.speculative_signed_step and paged.exact.
+// paged.speculative_step, paged.speculative_signed_step, paged.exact,
+// paged.extend, paged.attention and paged.shared_attention.
 //
 // A small step's kernel takes 5 us and its call from Python took 26 on the
 // host: about 6 us of checks, 10 of allocations, 4 of ctypes conversions and
@@ -12,9 +13,12 @@
 // addresses and which devices were prepared.
 #include <Python.h>
 
+#include <cmath>
+
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -29,7 +33,13 @@ struct Entry {
   decltype(&stk_paged_workspace_bytes) paged_workspace;
   decltype(&stk_paged_step) paged_step;
   decltype(&stk_paged_signed_step) paged_signed;
+  decltype(&stk_paged_extend) extend;
+  decltype(&stk_paged_attention_workspace_bytes) attention_workspace;
+  decltype(&stk_paged_attention) attention;
+  decltype(&stk_paged_shared_workspace_bytes) shared_workspace;
+  decltype(&stk_paged_shared_attention) shared;
 } g_entry;
+constexpr int kEntries = sizeof(Entry) / sizeof(void*);
 bool g_bound = false;
 uint64_t g_prepared = 0;   // bit per device whose step memory was looked up
 
@@ -40,15 +50,20 @@ const c10::DispatchKeySet kWrapped({c10::DispatchKey::FuncTorchBatched,
                                     c10::DispatchKey::ZeroTensor,
                                     c10::DispatchKey::NestedTensor});
 
-// A plain contiguous tensor on a GPU, or null.
-const at::Tensor* plain(PyObject* o) {
+// A plain tensor on a GPU, or null.
+const at::Tensor* plain_strided(PyObject* o) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided ||
-      t.key_set().has_any(kWrapped) || t.unsafeGetTensorImpl()->has_symbolic_sizes_strides() ||
-      !t.is_contiguous())
+      t.key_set().has_any(kWrapped) || t.unsafeGetTensorImpl()->has_symbolic_sizes_strides())
     return nullptr;
   return &t;
+}
+
+// A plain contiguous tensor on a GPU, or null.
+const at::Tensor* plain(PyObject* o) {
+  const at::Tensor* t = plain_strided(o);
+  return t && t->is_contiguous() ? t : nullptr;
 }
 
 bool no_modes() {
@@ -272,6 +287,213 @@ PyObject* paged_impl(PyObject* const* a, Py_ssize_t n) {
   return pack({&sel, &m, &l, &u, &out, &bad, &rem, &approx, &extra, &pos, &tot});
 }
 
+// The page pool of the dense operators: a[0..3 + bounds * 2) are K pages, V pages[,
+// lo, hi], table, nblocks; then ntokens or None.
+struct Pool {
+  const at::Tensor *k, *v, *lo, *hi, *table, *nblocks, *ntokens;
+  int64_t pages, b, d, r, hkv, width;
+  int dt;
+};
+
+bool int_vector(const at::Tensor& t, int64_t n) {
+  return t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n;
+}
+
+bool on(const at::Tensor* t, const at::Device& d) { return !t || t->device() == d; }
+
+bool pool_of(PyObject* const* a, bool bounds, Pool* p) {
+  const at::Tensor* t[7] = {};
+  const int n = bounds ? 6 : 4;
+  for (int i = 0; i < n; ++i)
+    if (!(t[i] = plain(a[i]))) return false;
+  if (a[n] != Py_None && !(t[6] = plain(a[n]))) return false;
+  p->k = t[0];
+  p->v = t[1];
+  p->lo = bounds ? t[2] : nullptr;
+  p->hi = bounds ? t[3] : nullptr;
+  p->table = t[n - 2];
+  p->nblocks = t[n - 1];
+  p->ntokens = t[6];
+  const at::Tensor &k = *p->k, &tab = *p->table;
+  p->dt = dtype_code(k);
+  if (p->dt < 0 || k.dim() != 3 || !small(k) || p->v->sizes() != k.sizes() ||
+      p->v->scalar_type() != k.scalar_type() || tab.dim() != 3 || !small(tab) ||
+      tab.scalar_type() != at::kInt)
+    return false;
+  p->pages = k.size(0);
+  p->b = k.size(1);
+  p->d = k.size(2);
+  p->r = tab.size(0);
+  p->hkv = tab.size(1);
+  p->width = tab.size(2);
+  if (!int_vector(*p->nblocks, p->r) || (p->ntokens && !int_vector(*p->ntokens, p->r)))
+    return false;
+  const auto dev = k.device();
+  if (dev.index() != c10::hip::current_device()) return false;
+  for (const at::Tensor* x : {p->v, p->lo, p->hi, p->table, p->nblocks, p->ntokens})
+    if (!on(x, dev)) return false;
+  if (!bounds) return true;
+  const at::Tensor &lo = *p->lo, &hi = *p->hi;
+  return lo.dim() == 2 && lo.size(0) == p->pages && lo.size(1) == p->d &&
+         hi.sizes() == lo.sizes() && hi.scalar_type() == lo.scalar_type() &&
+         (lo.scalar_type() == at::kFloat || lo.scalar_type() == k.scalar_type());
+}
+
+// Rows [T, heads, D] of the pool's type, contiguous within a token; *stride
+// from one token to the next.
+const at::Tensor* tokens_of(PyObject* o, const Pool& p, int64_t heads, int64_t* stride) {
+  const at::Tensor* t = plain_strided(o);
+  if (!t || t->dim() != 3 || !small(*t) || t->size(2) != p.d ||
+      (heads > 0 && t->size(1) != heads) || t->scalar_type() != p.k->scalar_type() ||
+      t->device() != p.k->device())
+    return nullptr;
+  const int64_t n = t->size(0), h = t->size(1);
+  if (t->stride(2) != 1 || (h > 1 && t->stride(1) != p.d) ||
+      (n > 1 && (t->stride(0) < h * p.d || t->stride(0) % 8)))
+    return nullptr;
+  *stride = n > 1 ? t->stride(0) : h * p.d;
+  return t;
+}
+
+bool disjoint(const at::Tensor& a, const at::Tensor* b) {
+  if (!b) return true;
+  const char* x = static_cast<const char*>(a.data_ptr());
+  const char* y = static_cast<const char*>(b->data_ptr());
+  return x + a.nbytes() <= y || y + b->nbytes() <= x;
+}
+
+const int32_t* ip(const at::Tensor* t) { return t ? t->data_ptr<int32_t>() : nullptr; }
+
+// (k_pages, v_pages, lo, hi, table, nblocks, ntokens or None, k_new, v_new,
+// starts, positions, cos, sin, q or None, interleaved): (rotated q or None,),
+// an error code, or None.  cos and sin may be None.
+PyObject* extend_impl(PyObject* const* a, Py_ssize_t n) {
+  Pool p;
+  if (!g_bound || n != 15 || !no_modes() || !pool_of(a, true, &p)) Py_RETURN_NONE;
+  int64_t ks, vs, qs = 0;
+  const at::Tensor* k = tokens_of(a[7], p, p.hkv, &ks);
+  const at::Tensor* v = tokens_of(a[8], p, p.hkv, &vs);
+  const at::Tensor *st = plain(a[9]), *pos = plain(a[10]);
+  if (!k || !v || k->size(0) != v->size(0) || !st || !pos || !int_vector(*st, p.r + 1) ||
+      !int_vector(*pos, p.r))
+    Py_RETURN_NONE;
+  const at::Tensor *co = nullptr, *si = nullptr, *q = nullptr;
+  const auto dev = p.k->device();
+  int64_t rows = 0, rot = 0, hq = 0;
+  if (a[11] != Py_None || a[12] != Py_None) {
+    co = plain(a[11]);
+    si = plain(a[12]);
+    if (!co || !si || co->dim() != 2 || !small(*co) || si->sizes() != co->sizes() ||
+        co->scalar_type() != at::kFloat || si->scalar_type() != at::kFloat)
+      Py_RETURN_NONE;
+    rows = co->size(0);
+    rot = 2 * co->size(1);
+  }
+  if (rot > p.d) Py_RETURN_NONE;
+  const int64_t t = k->size(0);
+  if (a[13] != Py_None) {
+    if (!co || !(q = tokens_of(a[13], p, 0, &qs)) || q->size(0) != t) Py_RETURN_NONE;
+    hq = q->size(1);
+  }
+  for (const at::Tensor* x : {st, pos, co, si})
+    if (!on(x, dev)) Py_RETURN_NONE;
+  if (!disjoint(*pos, p.ntokens) || !disjoint(*pos, p.nblocks)) Py_RETURN_NONE;
+  const int inter = PyObject_IsTrue(a[14]);
+  if (inter < 0) return nullptr;
+  at::Tensor out;
+  if (q) out = at::empty({t, hq, p.d}, p.k->options().requires_grad(false));
+  void* stream = stream_of(*p.k);
+  const int lb = p.lo->scalar_type() == at::kFloat ? 0 : p.dt;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_entry.extend(k->data_ptr(), ks, v->data_ptr(), vs, q ? q->data_ptr() : nullptr, qs,
+                      q ? out.data_ptr() : nullptr, p.dt, (int)t, (int)p.r, (int)hq, (int)p.hkv,
+                      (int)p.width, (int)p.b, (int)p.d, (int)p.pages, ip(st), ip(pos),
+                      co ? co->data_ptr<float>() : nullptr, si ? si->data_ptr<float>() : nullptr,
+                      (int)rows, (int)rot, inter, p.k->data_ptr(), p.v->data_ptr(),
+                      p.lo->data_ptr(), p.hi->data_ptr(), lb, ip(p.table),
+                      p.nblocks->data_ptr<int32_t>(),
+                      p.ntokens ? p.ntokens->data_ptr<int32_t>() : nullptr, stream);
+  Py_END_ALLOW_THREADS
+  if (rc) return PyLong_FromLong(rc);
+  return pack({&out});
+}
+
+// (k_pages, v_pages, table, nblocks, ntokens or None, q, starts, groups, shared, scale,
+// softcap, slopes, window, prefix, first, out): starts, groups and shared, scale,
+// slopes, prefix, first and out may be None.  Returns the output, an error code, or None.
+PyObject* attention_impl(PyObject* const* a, Py_ssize_t n) {
+  Pool p;
+  if (!g_bound || n != 16 || !no_modes() || !pool_of(a, false, &p)) Py_RETURN_NONE;
+  int64_t qs;
+  const at::Tensor* q = tokens_of(a[5], p, 0, &qs);
+  if (!q || q->size(1) % p.hkv) Py_RETURN_NONE;
+  const int64_t t = q->size(0), hq = q->size(1);
+  const at::Tensor* o[8] = {};                 // starts, groups, shared, slopes, prefix, first, out
+  const int at_[7] = {6, 7, 8, 11, 13, 14, 15};
+  for (int i = 0; i < 7; ++i)
+    if (a[at_[i]] != Py_None && (!(o[i] = plain(a[at_[i]])) || !on(o[i], p.k->device())))
+      Py_RETURN_NONE;
+  const at::Tensor *st = o[0], *gr = o[1], *sh = o[2], *slo = o[3], *pre = o[4], *fir = o[5];
+  double scale = 1.0 / std::sqrt((double)p.d), cap;
+  int window;
+  if ((a[9] != Py_None && !plain_float(a[9], &scale)) || !plain_float(a[10], &cap) ||
+      !plain_int(a[12], 0, 0x7fffffff, &window) || !(scale > 0) || !(cap >= 0) ||
+      std::isinf(scale) || std::isinf(cap))
+    Py_RETURN_NONE;
+  if ((st && !int_vector(*st, p.r + 1)) || (!st && t != p.r) || (pre && !int_vector(*pre, p.r)) ||
+      (fir && !int_vector(*fir, t)) ||
+      (slo && (slo->scalar_type() != at::kFloat || slo->dim() != 1 || slo->size(0) != hq)))
+    Py_RETURN_NONE;
+  int64_t ng = 0;
+  if (gr || sh) {
+    if (!gr || !sh || st || pre || gr->dim() != 1) Py_RETURN_NONE;
+    ng = gr->size(0) - 1;
+    if (ng < 1 || ng > p.r || !int_vector(*gr, ng + 1) || !int_vector(*sh, ng)) Py_RETURN_NONE;
+  }
+  if (o[6] && (o[6]->sizes() != q->sizes() || o[6]->scalar_type() != q->scalar_type()))
+    Py_RETURN_NONE;
+  const auto opt = q->options().requires_grad(false);
+  const at::Tensor out = o[6] ? *o[6] : at::empty({t, hq, p.d}, opt);
+  const size_t bytes =
+      ng ? g_entry.shared_workspace((int)p.r, (int)ng, (int)hq, (int)p.hkv, (int)p.width, (int)p.b,
+                                    (int)p.d)
+         : g_entry.attention_workspace((int)t, (int)p.r, (int)hq, (int)p.hkv, (int)p.width,
+                                       (int)p.b, (int)p.d, st != nullptr);
+  const at::Tensor ws = at::empty({(int64_t)(bytes ? bytes : 1)}, opt.dtype(at::kByte));
+  void* stream = stream_of(*q);
+  const float* slopes = slo ? slo->data_ptr<float>() : nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  if (ng)
+    rc = g_entry.shared(q->data_ptr(), qs, p.dt, (int)p.r, (int)hq, (int)p.hkv, (int)p.width,
+                        (int)p.b, (int)p.d, (int)p.pages, p.k->data_ptr(), p.v->data_ptr(),
+                        ip(p.table), ip(p.nblocks), ip(p.ntokens), ip(gr), ip(sh), (int)ng,
+                        (float)scale, (float)cap, slopes, window, ip(fir), out.data_ptr(),
+                        ws.data_ptr(), bytes, stream);
+  else
+    rc = g_entry.attention(q->data_ptr(), qs, p.dt, (int)t, (int)p.r, (int)hq, (int)p.hkv,
+                           (int)p.width, (int)p.b, (int)p.d, (int)p.pages, p.k->data_ptr(),
+                           p.v->data_ptr(), ip(p.table), ip(p.nblocks), ip(p.ntokens), ip(st),
+                           (float)scale, (float)cap, slopes, window, ip(pre), ip(fir),
+                           out.data_ptr(), o[6] == nullptr, ws.data_ptr(), bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (rc) return PyLong_FromLong(rc);
+  if (o[6]) {
+    Py_INCREF(a[15]);
+    return a[15];
+  }
+  return THPVariable_Wrap(out);
+}
+
+PyObject* paged_extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return checked([&] { return extend_impl(a, n); });
+}
+
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return checked([&] { return attention_impl(a, n); });
+}
+
 PyObject* speculative_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return checked([&] { return step_impl(a, n); });
 }
@@ -280,15 +502,14 @@ PyObject* paged_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return checked([&] { return paged_impl(a, n); });
 }
 
-// bind(step_supported, step_workspace, step, paged_workspace, paged_step,
-// paged_signed): the C entry points' addresses
+// bind(...): the addresses of Entry's C entry points, in its order
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 6) {
-    PyErr_SetString(PyExc_TypeError, "bind takes six addresses");
+  if (n != kEntries) {
+    PyErr_Format(PyExc_TypeError, "bind takes %d addresses", kEntries);
     return nullptr;
   }
-  void* p[6];
-  for (int i = 0; i < 6; ++i) {
+  void* p[kEntries];
+  for (int i = 0; i < kEntries; ++i) {
     p[i] = PyLong_AsVoidPtr(a[i]);
     if (!p[i]) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null address");
@@ -309,6 +530,8 @@ PyObject* prepared(PyObject*, PyObject* o) {
 PyMethodDef kMethods[] = {
     {"speculative_step", (PyCFunction)(void (*)())speculative_step, METH_FASTCALL, nullptr},
     {"paged_step", (PyCFunction)(void (*)())paged_step, METH_FASTCALL, nullptr},
+    {"paged_extend", (PyCFunction)(void (*)())paged_extend, METH_FASTCALL, nullptr},
+    {"paged_attention", (PyCFunction)(void (*)())paged_attention, METH_FASTCALL, nullptr},
     {"bind", (PyCFunction)(void (*)())bind, METH_FASTCALL, nullptr},
     {"prepared", (PyCFunction)prepared, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -136,11 +136,11 @@ class _PythonOnly:
     def speculative_step(self, *args):
         return None
 
-    paged_step = prepared = speculative_step
+    paged_step = paged_extend = paged_attention = prepared = speculative_step
 
 
 def host():
-    """The native host path of the fused steps (csrc/host.cpp): its functions
+    """The native host path of the fused steps and the dense operators (csrc/host.cpp): its functions
     return None for calls that the Python code has to check or refuse.  The
     module is built for one Python and one torch; without one for this process
     the steps run through the Python code alone, whose results are the same."""
@@ -153,7 +153,9 @@ def host():
                 raise ImportError(f"built for torch {module.torch_version}")
             module.bind(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in (
                 "stk_step_supported", "stk_step_workspace_bytes", "stk_speculative_step",
-                "stk_paged_workspace_bytes", "stk_paged_step", "stk_paged_signed_step")))
+                "stk_paged_workspace_bytes", "stk_paged_step", "stk_paged_signed_step",
+                "stk_paged_extend", "stk_paged_attention_workspace_bytes", "stk_paged_attention",
+                "stk_paged_shared_workspace_bytes", "stk_paged_shared_attention")))
         except ImportError as e:
             warnings.warn(f"strict_topk native host module not used ({e}): the fused steps cost "
                           "more host time; build it with `python strict-topk-overlap_amd/"

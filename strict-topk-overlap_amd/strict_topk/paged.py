@@ -256,6 +256,14 @@ def extend(kv, k_new, v_new, starts, positions, cos=None, sin=None, q=None, inte
     not written, and their request keeps its counts.  Tokens may lie
     apart (views of one fused projection), heads and dims must not.  All
     lengths stay on the device, so a captured graph follows them."""
+    if type(kv) is PagedKV:
+        got = _lib.host().paged_extend(kv.k_pages, kv.v_pages, kv.lo_pages, kv.hi_pages,
+                                       kv.block_table, kv.nblocks, kv.ntokens, k_new, v_new,
+                                       starts, positions, cos, sin, q, interleaved)
+        if type(got) is int:
+            _lib.fail(got)
+        if got is not None:
+            return got[0]
     dev = _check_pool(kv, True)
     r, hkv = kv.requests, kv.hkv
     ks = _check_tokens("K_NEW", k_new, kv, hkv)
@@ -327,6 +335,20 @@ def _dense_args(q, kv, scale, softcap, slopes, window, first, out):
     return dev, qs, t, hq, d, scale, softcap, window, res
 
 
+def _native_dense(q, kv, starts, groups, shared, scale, softcap, slopes, window, prefix, first,
+                  out):
+    """``attention`` or (with groups) ``shared_attention`` on the native host path, or None where
+    the code below has to check or refuse the call."""
+    if type(kv) is not PagedKV:
+        return None
+    got = _lib.host().paged_attention(kv.k_pages, kv.v_pages, kv.block_table, kv.nblocks,
+                                      kv.ntokens, q, starts, groups, shared, scale, softcap,
+                                      slopes, window, prefix, first, out)
+    if type(got) is int:
+        _lib.fail(got)
+    return got
+
+
 def attention(q, kv, starts=None, scale=None, softcap=0.0, slopes=None, window=0, prefix=None,
               first=None, out=None):
     """Dense attention of each request's newest tokens over its whole cache.
@@ -351,6 +373,10 @@ def attention(q, kv, starts=None, scale=None, softcap=0.0, slopes=None, window=0
     that belong to no request (padding) come back zero, or with ``out`` are left
     as they were.  Tokens of q may lie apart, heads and dims must not.  All lengths
     stay on the device, so a captured graph follows them."""
+    got = _native_dense(q, kv, starts, None, None, scale, softcap, slopes, window, prefix, first,
+                        out)
+    if got is not None:
+        return got
     dev, qs, t, hq, d, scale, softcap, window, res = _dense_args(
         q, kv, scale, softcap, slopes, window, first, out)
     r = kv.requests
@@ -384,11 +410,18 @@ def shared_attention(q, kv, groups, shared, scale=None, softcap=0.0, slopes=None
     and multiplied with all its queries together, the rest per request, and the
     two parts joined.  Requests outside every group share nothing.  The other
     arguments and the result are those of ``attention``."""
+    if groups is not None and shared is not None:
+        got = _native_dense(q, kv, None, groups, shared, scale, softcap, slopes, window, None,
+                            first, out)
+        if got is not None:
+            return got
     dev, qs, t, hq, d, scale, softcap, window, res = _dense_args(
         q, kv, scale, softcap, slopes, window, first, out)
     r = kv.requests
     if t != r:
         raise ValueError("expected one query token per request")
+    if groups is None or shared is None:
+        raise ValueError("expected int32 groups[G+1] and shared[G]")
     if groups.ndim != 1 or not 2 <= groups.shape[0] <= r + 1:
         raise ValueError("expected int32 groups[G+1], 1 <= G <= R")
     n = groups.shape[0] - 1

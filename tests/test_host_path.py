@@ -182,3 +182,68 @@ def test_paged_equals_the_python_path(monkeypatch, tokens):
         paged.speculative_step(q, kv, p, 257)
     with pytest.raises(ValueError, match="int32"):
         paged.speculative_step(q, kv, p.long(), 7)
+
+
+def _dense_calls(dev):
+    """Calls of the dense operators: (function, arguments) over one pool."""
+    from strict_topk import paged
+    from tests import dense_ref as R
+    kv = R.make(2, 64, 16, [40, 20, 33], torch.bfloat16, device=dev)
+    fused = R.queries(9, 8, 64, torch.bfloat16, device=dev)
+    q, k, v = fused[:, :4], fused[:, 4:6], fused[:, 6:]
+    ints = dict(dtype=torch.int32, device=dev)
+    cos, sin = R.tables(kv.width * 16, 32, device=dev)
+    starts, pos = torch.tensor([0, 2, 2, 9], **ints), torch.tensor([3, 5, 20], **ints)
+    one = torch.empty((3, 4, 64), dtype=torch.bfloat16, device=dev)
+    groups, shared = torch.tensor([0, 2], **ints), torch.tensor([0], **ints)
+    return [
+        (paged.extend, (kv, k, v, starts, pos), {}),
+        (paged.extend, (kv, k, v, starts, pos, cos, sin), dict(q=q, interleaved=True)),
+        (paged.attention, (q[:3], kv), {}),
+        (paged.attention, (q[:3], kv), dict(out=one, scale=1, softcap=5.0, window=9)),
+        (paged.attention, (q, kv, starts), dict(slopes=R.slopes_of(4, dev),
+                                                prefix=torch.tensor([1, 2, 3], **ints),
+                                                first=torch.arange(9, **ints))),
+        (paged.shared_attention, (q[:3], kv, groups, shared), dict(first=pos))]
+
+
+def test_dense_calls_on_the_cpu_are_declined_and_refused():
+    from strict_topk import _lib
+    host = _lib.host()
+    assert host.paged_extend(*[None] * 15) is None and host.paged_extend() is None
+    assert host.paged_attention(*[None] * 16) is None and host.paged_attention(1, 2) is None
+    for fn, args, kw in _dense_calls("cpu"):
+        with pytest.raises(ValueError, match="CUDA device"):
+            fn(*args, **kw)
+
+
+@pytest.mark.gpu
+def test_dense_calls_equal_the_python_path(monkeypatch):
+    """Both paths' results are the same bits, and the native path takes every plain call."""
+    from strict_topk import _lib
+    taken = []
+    host = _lib.host()
+
+    class Counted:
+        def __getattr__(self, name):
+            def call(*a):
+                got = getattr(host, name)(*a)
+                taken.append(got is not None)
+                return got
+            return call
+
+    def results():
+        out = []
+        for fn, args, kw in _dense_calls(DEV):
+            got = fn(*args, **kw)
+            kv = next(x for x in args if hasattr(x, "k_pages"))
+            out += [None if got is None else got.clone(), kv.k_pages, kv.v_pages, kv.lo_pages,
+                    kv.hi_pages, kv.nblocks, kv.ntokens]
+        return out
+
+    monkeypatch.setattr(_lib, "_host", Counted())
+    native = results()
+    assert len(taken) == 6 and all(taken)
+    monkeypatch.setattr(_lib, "_host", _lib._PythonOnly())
+    for a, b in zip(native, results()):
+        assert (a is None) == (b is None) and (a is None or torch.equal(a, b))

@@ -1,6 +1,6 @@
 // Dense attention over the paged cache: the C entry points, the list of row
 // tiles (k_plan), and the joins of split items (k_join_tiles, k_join_rows).
-#include "dense_decode.hpp"
+#include "dense_shared.hpp"
 
 namespace stk {
 
@@ -120,9 +120,35 @@ __global__ __launch_bounds__(256) void k_join_tiles(DenseArgs a, Plan pl, Parts 
   }
 }
 
+// Joins `count` parts of one row into (m, l, o): rows `pr` of slot(i), four columns per
+// thread.  Four parts at a time, their loads in flight together.
+template <typename F>
+__device__ __forceinline__ void join_parts(const Parts& p, int i0, int count, int step, int d,
+                                           int col, F row, float& m, float& l, f32x4& o) {
+  for (int i = i0; i < count; i += 4 * step) {
+    float pm[4], plx[4];
+    f32x4 po[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int64_t r = row(min(i + x * step, count - 1));
+      pm[x] = p.m[r];
+      plx[x] = p.l[r];
+      po[x] = *reinterpret_cast<const f32x4*>(p.o + r * d + col);
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (i + x * step >= count) break;
+      const float mx = fmaxf(m, pm[x]), f = part_weight(m, mx), fi = part_weight(pm[x], mx);
+      m = mx;
+      l = l * f + plx[x] * fi;
+      o = o * f + po[x] * fi;
+    }
+  }
+}
+
 // One (request, query head) of a decode batch: the parts of its own keys, and
-// with groups those of the shared keys.
-template <typename T, int D>
+// with SHARED those of its group's shared keys.
+template <typename T, int D, bool SHARED>
 __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Parts whole,
                                                    const int32_t* place, int launched, Plan pl,
                                                    Parts psplit, Parts pwhole, int plaunched) {
@@ -132,57 +158,43 @@ __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Par
   const int r = (int)blockIdx.x / a.hq, head = (int)blockIdx.x % a.hq;
   const int kvh = head / a.g, gi = head % a.g, nc = decode_chunks(a);
   const int item = kvh * nc + gi / kDecodeRows, hrow = gi % kDecodeRows;
-  // a request's span is one unit or more for each of its items
-  const int base = place[r], total = place[a.requests];
-  const int n = (place[r + 1] - base) / (a.hkv * nc), first = base + item * n;
+  const int dc = threadIdx.x % CH, grp = threadIdx.x / CH;
+  // a request has the same units for each of its items
+  const int base = place[r], end = place[r + 1], total = place[a.requests];
+  const int n = (end - base) / (a.hkv * nc), first = base + item * n;
   const Deal deal(total, launched);
   const int w0 = deal.wg_of(first), w1 = deal.wg_of(first + n - 1);
-  const int ns = w1 - w0 + 1;
-  int np = 0, v0 = 0, rr = 0;
-  int64_t pslot = 0;
-  if (a.groups) {
+  float m = -INFINITY, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  if (w0 == w1) {
+    if constexpr (!SHARED) return;               // finished by its workgroup
+    const int64_t at = ((int64_t)r * a.hkv * nc + item) * kDecodeRows + hrow;
+    join_parts(whole, grp, 1, NP, D, 4 * dc, [&](int) { return at; }, m, l, o);
+  } else {
+    join_parts(split, grp, w1 - w0 + 1, NP, D, 4 * dc, [&](int i) {
+      return (2 * (int64_t)(w0 + i) + (i == 0 ? 1 : 0)) * kDecodeRows + hrow;
+    }, m, l, o);
+  }
+  if constexpr (SHARED) {
     const int g = group_of(a, r);
     if (g >= 0) {
       int s0, s1;
       seq_rows(a, g, s0, s1);
       const int64_t idx = (int64_t)(r - s0) * a.g + gi;
-      const int tile = (int)(idx / kDenseRows), it = pl.base[g + 1] - 1 - tile;
-      rr = (int)(idx % kDenseRows);
-      const int per = pl.head[0], ntiles = pl.head[1];
-      const int cum = pl.tiles[it].cum;
-      const int pn = (it + 1 < ntiles ? pl.tiles[it + 1].cum : per) - cum;
+      const int tile = (int)(idx / kDenseRows), rr = (int)(idx % kDenseRows);
+      const int units = group_units(a, g, kTk<D>), per = pl.base[a.ngroups];
+      const int pf = kvh * per + pl.base[g] + tile * units;
       const Deal pdeal(per * a.hkv, plaunched);
-      v0 = pdeal.wg_of(kvh * per + cum);
-      np = pdeal.wg_of(kvh * per + cum + pn - 1) - v0 + 1;
-      pslot = (int64_t)kvh * ntiles + it;
+      const int v0 = pdeal.wg_of(pf), v1 = pdeal.wg_of(pf + units - 1);
+      if (v0 == v1) {
+        const int64_t at = group_slot(a, kvh, g, s0, tile, pl.limit) * kDenseRows + rr;
+        join_parts(pwhole, grp, 1, NP, D, 4 * dc, [&](int) { return at; }, m, l, o);
+      } else {
+        join_parts(psplit, grp, v1 - v0 + 1, NP, D, 4 * dc, [&](int i) {
+          return (2 * (int64_t)(v0 + i) + (i == 0 ? 1 : 0)) * kDenseRows + rr;
+        }, m, l, o);
+      }
     }
-  } else if (ns == 1) {
-    return;                                      // finished by its workgroup
-  }
-  const int dc = threadIdx.x % CH, grp = threadIdx.x / CH;
-  float m = -INFINITY, l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int i = grp; i < ns + np; i += NP) {
-    const float *pm, *pl_, *po;
-    int64_t pr;
-    if (i < ns) {
-      const Parts& from = ns == 1 ? whole : split;
-      pr = (ns == 1 ? (int64_t)r * a.hkv * nc + item : 2 * (int64_t)(w0 + i) + (i == 0 ? 1 : 0)) *
-               kDecodeRows + hrow;
-      pm = from.m; pl_ = from.l; po = from.o;
-    } else {
-      const int q = i - ns;
-      const Parts& from = np == 1 ? pwhole : psplit;
-      pr = (np == 1 ? pslot : 2 * (int64_t)(v0 + q) + (q == 0 ? 1 : 0)) * kDenseRows + rr;
-      pm = from.m; pl_ = from.l; po = from.o;
-    }
-    const float mi = pm[pr], li = pl_[pr], mx = fmaxf(m, mi);
-    const f32x4 oi = *reinterpret_cast<const f32x4*>(po + pr * D + 4 * dc);
-    const float f = part_weight(m, mx), fi = part_weight(mi, mx);
-    m = mx;
-    l = l * f + li * fi;
-    o = o * f + oi * fi;
   }
   if (dc == 0) {
     s_m[grp] = m;
@@ -191,6 +203,7 @@ __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Par
   s_o[grp][dc] = o;
   __syncthreads();
   if (grp == 0) {
+#pragma unroll
     for (int i = 1; i < NP; ++i) {
       const float mi = s_m[i], mx = fmaxf(m, mi);
       const float f = part_weight(m, mx), fi = part_weight(mi, mx);
@@ -243,6 +256,13 @@ static int64_t prefill_units(const DenseShape& s) {
   const int tk = s.d == 256 ? 32 : 64;
   return tile_limit(s) * s.hkv * (((int64_t)s.nb * s.b + tk - 1) / tk + 1);
 }
+// The most units that a launch counts.  Groups come from the device: even if all
+// of them held all requests, their units would have to fit an int.
+static int64_t most_units(const DenseShape& s) {
+  if (!s.ngroups) return prefill_units(s);
+  const int64_t rows = (int64_t)s.requests * (s.hq / s.hkv);
+  return (prefill_units(s) / tile_limit(s)) * (rows / kDenseRows + 1) * s.ngroups;
+}
 // Tiles that fill the device several times over need no splitting, and neither do
 // those of caches that hold few units: without it there is nothing to list and
 // nothing to join.
@@ -270,18 +290,18 @@ static Parts take_parts(Carve& c, int64_t slots, int rows, int d) {
   p.o = c.take<float>((size_t)slots * rows * d);
   return p;
 }
+// With groups there is no list of tiles: only the units before each group are kept.
 static size_t plan_bytes(const DenseShape& s) {
-  const int ns = s.ngroups ? s.ngroups : s.requests;
-  return stk_align(2 * sizeof(int32_t)) + stk_align((ns + 1) * sizeof(int32_t)) +
+  if (s.ngroups) return stk_align((s.ngroups + 1) * sizeof(int32_t));
+  return stk_align(2 * sizeof(int32_t)) + stk_align((s.requests + 1) * sizeof(int32_t)) +
          stk_align((size_t)tile_limit(s) * sizeof(Tile));
 }
 static Plan take_plan(Carve& c, const DenseShape& s) {
-  const int ns = s.ngroups ? s.ngroups : s.requests;
-  Plan p;
-  p.head = c.take<int32_t>(2);
-  p.base = c.take<int32_t>(ns + 1);
+  Plan p{};
   p.limit = (int)tile_limit(s);
-  p.tiles = c.take<Tile>(p.limit);
+  if (!s.ngroups) p.head = c.take<int32_t>(2);
+  p.base = c.take<int32_t>((s.ngroups ? s.ngroups : s.requests) + 1);
+  if (!s.ngroups) p.tiles = c.take<Tile>(p.limit);
   return p;
 }
 
@@ -316,14 +336,13 @@ static void launch_join_tiles(const DenseArgs& a, const Plan& p, const Parts& sp
   else hipLaunchKernelGGL((k_join_tiles<T, 256>), g, dim3(256), 0, st, a, p, split, grid);
 }
 
-template <typename T>
+template <typename T, bool SHARED>
 static void launch_join_rows(const DenseArgs& a, const Parts& split, const Parts& whole,
-                             const int32_t* place, int grid, const Plan& p, const Parts& ps, const Parts& pw, int pgrid, int d,
-                             hipStream_t st) {
-  const dim3 g((unsigned)(a.requests * a.hq));
+                             const int32_t* place, int grid, const Plan& p, const Parts& ps,
+                             const Parts& pw, int pgrid, int d, hipStream_t st) {
+  const unsigned g = (unsigned)(a.requests * a.hq);
 #define STK_JOIN(D) \
-  hipLaunchKernelGGL((k_join_rows<T, D>), g, dim3(256), 0, st, a, split, whole, place, \
-                     grid, p, ps, pw, pgrid)
+  k_join_rows<T, D, SHARED><<<g, 256, 0, st>>>(a, split, whole, place, grid, p, ps, pw, pgrid)
   if (d == 64) STK_JOIN(64);
   else if (d == 128) STK_JOIN(128);
   else STK_JOIN(256);
@@ -333,16 +352,14 @@ static void launch_join_rows(const DenseArgs& a, const Parts& split, const Parts
 template <typename T>
 static int run_dense(const DenseShape& s, DenseArgs a, int mode, void* workspace, hipStream_t st) {
   Carve c(workspace);
-  const Parts none{nullptr, nullptr, nullptr};
   if (s.ragged) {
     const int grid = prefill_grid(s);
-    if (prefill_direct(s))
-      return launch_prefill<T>(s.d, mode, a, Plan{}, none, none, grid, true, st);
+    if (prefill_direct(s)) return launch_direct<T>(s.d, mode, a, grid, st);
     const Plan p = take_plan(c, s);
     const Parts split = take_parts(c, 2 * (int64_t)grid, kDenseRows, s.d);
     int rc = launch_plan(a, p, s.d, st);
     if (rc) return rc;
-    rc = launch_prefill<T>(s.d, mode, a, p, split, none, grid, false, st);
+    rc = launch_prefill<T>(s.d, mode, a, p, split, grid, st);
     if (rc) return rc;
     launch_join_tiles<T>(a, p, split, grid, s.d, st);
     return stk_check_launch("k_join_tiles");
@@ -351,23 +368,21 @@ static int run_dense(const DenseShape& s, DenseArgs a, int mode, void* workspace
   const int grid = decode_grid(s);
   int32_t* place = c.take<int32_t>(s.requests + 1);
   const Parts split = take_parts(c, 2 * (int64_t)grid, kDecodeRows, s.d);
-  Parts whole = none, ps = none, pw = none;
-  Plan p{};
-  int pgrid = 0;
   if (s.ngroups) {
-    whole = take_parts(c, (int64_t)s.requests * s.hkv * nc, kDecodeRows, s.d);
-    p = take_plan(c, s);
-    pgrid = prefill_grid(s);
-    ps = take_parts(c, 2 * (int64_t)pgrid, kDenseRows, s.d);
-    pw = take_parts(c, tile_limit(s) * s.hkv, kDenseRows, s.d);
-    int rc = launch_plan(a, p, s.d, st);
+    const Parts whole = take_parts(c, (int64_t)s.requests * s.hkv * nc, kDecodeRows, s.d);
+    const Plan p = take_plan(c, s);
+    const int pgrid = prefill_grid(s);
+    const Parts ps = take_parts(c, 2 * (int64_t)pgrid, kDenseRows, s.d);
+    const Parts pw = take_parts(c, tile_limit(s) * s.hkv, kDenseRows, s.d);
+    const int rc = launch_shared<T>(s.d, mode, a, p, ps, pw, pgrid, split, whole, place, grid, st);
     if (rc) return rc;
-    rc = launch_prefill<T>(s.d, mode, a, p, ps, pw, pgrid, false, st);
+    launch_join_rows<T, true>(a, split, whole, place, grid, p, ps, pw, pgrid, s.d, st);
+  } else {
+    const int rc = launch_decode<T>(s.d, mode, a, split, place, grid, st);
     if (rc) return rc;
+    launch_join_rows<T, false>(a, split, Parts{}, place, grid, Plan{}, Parts{}, Parts{}, 0, s.d,
+                               st);
   }
-  int rc = launch_decode<T>(s.d, mode, a, split, whole, place, grid, st);
-  if (rc) return rc;
-  launch_join_rows<T>(a, split, whole, place, grid, p, ps, pw, pgrid, s.d, st);
   return stk_check_launch("k_join_rows");
 }
 
@@ -390,7 +405,7 @@ static int dense(const DenseShape& s, const void* q, int64_t q_stride, int dtype
                15) == 0 && q_stride % 8 == 0 && q_stride >= 0,
               "rows must be 16-byte aligned");
   STK_REQUIRE(decode_units(s) <= 0x7fffffff && (int64_t)s.requests * s.hq <= 0x7fffffff &&
-                  prefill_units(s) <= 0x7fffffff,
+                  most_units(s) <= 0x7fffffff,
               "batch too large");
   STK_REQUIRE(workspace && workspace_bytes >= dense_bytes(s), "workspace too small");
   STK_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0,

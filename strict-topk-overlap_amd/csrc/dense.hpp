@@ -235,12 +235,18 @@ __device__ __forceinline__ Span seq_span(const DenseArgs& a, int q, int s0, int 
   return span_of(a, q, t, p, n);
 }
 
-// dense_decode_*.hip, dense_prefill_*.hip: one element type each
+// dense_*_{bf16,f16}.hip: one element type each
 template <typename T>
-int launch_decode(int d, int mode, const DenseArgs& a, const Parts& split, const Parts& whole,
+int launch_decode(int d, int mode, const DenseArgs& a, const Parts& split, int32_t* place, int grid,
+                  hipStream_t st);
+template <typename T>
+int launch_prefill(int d, int mode, const DenseArgs& a, const Plan& p, const Parts& split, int grid,
+                   hipStream_t st);
+template <typename T>
+int launch_direct(int d, int mode, const DenseArgs& a, int grid, hipStream_t st);
+template <typename T>
+int launch_shared(int d, int mode, const DenseArgs& a, const Plan& p, const Parts& psplit,
+                  const Parts& pwhole, int pgrid, const Parts& split, const Parts& whole,
                   int32_t* place, int grid, hipStream_t st);
-template <typename T>
-int launch_prefill(int d, int mode, const DenseArgs& a, const Plan& p, const Parts& split,
-                   const Parts& whole, int grid, bool direct, hipStream_t st);
 
 }  // namespace stk

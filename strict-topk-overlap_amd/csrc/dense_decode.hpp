@@ -94,29 +94,33 @@ __device__ __forceinline__ DecodePlace decode_place(const DenseArgs& a, int wg, 
   return p;
 }
 
-template <typename T, int D, int MODE>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_decode(DenseArgs a, Parts split, Parts whole,
-                                                   int32_t* place) {
+template <int D> constexpr size_t kDecodeLds = 4 * sizeof(uint16_t) * 32 * D;
+
+// The work of workgroup wg of nwg.  With PARTS items that lie whole in it leave
+// their parts in `whole`, too, instead of being finished.
+template <typename T, int D, int MODE, bool PARTS>
+__device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, const Parts& whole,
+                                       int32_t* place, char* lds, int wg, int nwg) {
   constexpr int KS = D / 32;            // QK steps
   constexpr int DB = D / 16;            // output blocks
   constexpr int VN = D / 16;            // 16-byte chunks of a V tile per lane
   constexpr int CPR = D / 8;            // chunks per row
   constexpr int RPI = STK_WAVE / CPR;   // rows per load instruction
-  __shared__ __attribute__((aligned(16))) uint16_t s_v[4][32 * D];
+  uint16_t* const s_v = reinterpret_cast<uint16_t*>(lds);         // [4][32 * D]
   __shared__ float s_m[4][16], s_l[4][16];
   const int lane = lane_id(), w = wave_id();
   const int n16 = lane & 15, kg = lane >> 4;
   const int nc = decode_chunks(a);
-  const DecodePlace at = decode_place(a, (int)blockIdx.x, (int)gridDim.x, place);
-  const Deal deal(at.total, (int)gridDim.x);
-  if (blockIdx.x >= deal.grid) return;
-  int u = deal.at((int)blockIdx.x);
-  const int u1 = deal.at((int)blockIdx.x + 1);
+  const DecodePlace at = decode_place(a, wg, nwg, place);
+  const Deal deal(at.total, nwg);
+  if ((uint32_t)wg >= deal.grid) return;
+  int u = deal.at(wg);
+  const int u1 = deal.at(wg + 1);
   int r = at.r, base = at.base;
   // V tile in LDS: row-major, 32-byte blocks swizzled so that the 16 rows of a
   // transposed read spread over all banks
   auto fsw = [](int row) { return D == 64 ? (row >> 1) & 3 : row & 7; };
-  uint16_t* vt = s_v[w];
+  uint16_t* vt = s_v + w * (32 * D);
   int vw[VN], va[DB];
 #pragma unroll
   for (int i = 0; i < VN; ++i) {
@@ -276,10 +280,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_decode(DenseArgs a, P
     }
     __syncthreads();
     const bool all = j0 == 0 && j1 == sp.n;
-    const bool keep = all && !whole.m;                  // finished here
+    const bool keep = all && !PARTS;                    // finished here
     const Parts& to = all ? whole : split;
     const int64_t slot = all ? (int64_t)r * a.hkv * nc + item
-                             : 2 * (int64_t)blockIdx.x + (j0 > 0 ? 0 : 1);
+                             : 2 * (int64_t)wg + (j0 > 0 ? 0 : 1);
     for (int x = threadIdx.x; x < gn * (D / 4); x += 256) {
       const int h = x / (D / 4), dc = x % (D / 4);
       float mx = s_m[0][h];
@@ -292,8 +296,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_decode(DenseArgs a, P
         const float mi = s_m[i][h];
         const float f = part_weight(mi, mx);
         sum += f * s_l[i][h];
-        o += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(s_v[i]) + h * D +
-                                                 4 * dc);
+        o += f * *reinterpret_cast<const f32x4*>(
+                     reinterpret_cast<const float*>(s_v + i * (32 * D)) + h * D + 4 * dc);
       }
       if (keep) {
         store_out<T>(a.out + ((int64_t)r * a.hq + h0 + h) * D + 4 * dc, o, sum);
@@ -308,6 +312,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_decode(DenseArgs a, P
     }
     __syncthreads();
   }
+}
+
+template <typename T, int D, int MODE>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_decode(DenseArgs a, Parts split,
+                                                                  int32_t* place) {
+  __shared__ __attribute__((aligned(16))) char lds[kDecodeLds<D>];
+  decode<T, D, MODE, false>(a, split, split, place, lds, (int)blockIdx.x, (int)gridDim.x);
 }
 
 }  // namespace stk

@@ -1,21 +1,17 @@
-// Dense decode attention, BF16 (dense_decode.hpp).
+// Dense decode attention, BF16 (k_decode).
 #include "dense_decode.hpp"
 
 namespace stk {
 
 template <>
-int launch_decode<bf16s>(int d, int mode, const DenseArgs& a, const Parts& split, const Parts& whole,
-                         int32_t* place, int grid, hipStream_t st) {
-#define STK_MODE(D)                                                                            \
-  switch (mode) {                                                                              \
-    case 0: hipLaunchKernelGGL((k_decode<bf16s, D, 0>), dim3(grid), dim3(256), 0, st, a, split, \
-                               whole, place); break;                                           \
-    case 1: hipLaunchKernelGGL((k_decode<bf16s, D, 1>), dim3(grid), dim3(256), 0, st, a, split, \
-                               whole, place); break;                                           \
-    case 2: hipLaunchKernelGGL((k_decode<bf16s, D, 2>), dim3(grid), dim3(256), 0, st, a, split, \
-                               whole, place); break;                                           \
-    default: hipLaunchKernelGGL((k_decode<bf16s, D, 3>), dim3(grid), dim3(256), 0, st, a,       \
-                                split, whole, place);                                          \
+int launch_decode<bf16s>(int d, int mode, const DenseArgs& a, const Parts& split, int32_t* place,
+                      int grid, hipStream_t st) {
+#define STK_MODE(D)                                                                \
+  switch (mode) {                                                                  \
+    case 0: k_decode<bf16s, D, 0><<<grid, 256, 0, st>>>(a, split, place); break;   \
+    case 1: k_decode<bf16s, D, 1><<<grid, 256, 0, st>>>(a, split, place); break;   \
+    case 2: k_decode<bf16s, D, 2><<<grid, 256, 0, st>>>(a, split, place); break;   \
+    default: k_decode<bf16s, D, 3><<<grid, 256, 0, st>>>(a, split, place); break;  \
   }
   if (d == 64) {
     STK_MODE(64)

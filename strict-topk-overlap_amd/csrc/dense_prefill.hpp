@@ -54,7 +54,7 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 // hidden keys and their values are not read.
 template <typename T, int D, int MODE>
 __device__ void slow_rows(const DenseArgs& a, int seq, int s0, int s1, int64_t rown, int kvh,
-                          const int32_t* row, int kbase, int kend, const Parts& to, int64_t pr) {
+                          const int32_t* row, int kbase, int kend, const Parts* to, int64_t pr) {
   constexpr int E = D / STK_WAVE;
   const int lane = lane_id();
   for (int i = 0; i < 32; ++i, ++rown, ++pr) {
@@ -93,12 +93,12 @@ __device__ void slow_rows(const DenseArgs& a, int seq, int s0, int s1, int64_t r
           o[x] += ek * cvt(T{a.vp[(int64_t)rk * D + lane + STK_WAVE * x]});
       }
     }
-    if (to.m) {
+    if (to) {
 #pragma unroll
-      for (int x = 0; x < E; ++x) to.o[pr * D + lane + STK_WAVE * x] = o[x];
+      for (int x = 0; x < E; ++x) to->o[pr * D + lane + STK_WAVE * x] = o[x];
       if (lane == 0) {
-        to.m[pr] = m;
-        to.l[pr] = l;
+        to->m[pr] = m;
+        to->l[pr] = l;
       }
     } else {
       const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -114,7 +114,7 @@ __device__ void slow_rows(const DenseArgs& a, int seq, int s0, int s1, int64_t r
 // which see the most keys, first.  kvh = Hkv: none.
 struct TilePlace { int seq, tile, kvh; };
 
-__device__ __forceinline__ TilePlace tile_place(const DenseArgs& a, int wg) {
+__device__ __forceinline__ TilePlace tile_place(const DenseArgs& a, int wg, int nwg) {
   __shared__ int s_tmp[4], s_at[2];
   const int ns = sequences(a);
   auto tiles = [&](int q) {
@@ -127,7 +127,7 @@ __device__ __forceinline__ TilePlace tile_place(const DenseArgs& a, int wg) {
     const int c = tiles(q0 + (int)threadIdx.x);
     int sum;
     __syncthreads();
-    const int before = block_excl_scan1(c, s_tmp, &sum);
+    const int before = block_excl_scan1(c, s_tmp, &sum);   // (of the first 256: from 0)
     if (q0 == 0) {
       c0 = c;
       b0 = before;
@@ -135,7 +135,7 @@ __device__ __forceinline__ TilePlace tile_place(const DenseArgs& a, int wg) {
     }
     total += sum;
   }
-  const int64_t all = min((int64_t)total * a.hkv, (int64_t)gridDim.x);
+  const int64_t all = min((int64_t)total * a.hkv, (int64_t)nwg);
   if (wg >= all) return TilePlace{0, 0, a.hkv};
   const int x = xcd_remap(wg, (int)all), kvh = x / total, it = x % total;
   int base = 0;
@@ -157,10 +157,73 @@ __device__ __forceinline__ TilePlace tile_place(const DenseArgs& a, int wg) {
                    __builtin_amdgcn_readfirstlane(s_at[1]), kvh};
 }
 
-template <typename T, int D, int MODE>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, Plan pl,
-                                                                   Parts split, Parts whole,
-                                                                   int direct) {
+// Shared blocks: every tile of a group has the same units, those of its
+// shared blocks.  The units of the groups' tiles end to end, per KV head: how many
+// there are, the group that holds unit u (taken modulo them), and the units before
+// it.  Workgroup 0 also leaves the units before every group, and their total, in
+// place [groups + 1] for k_join_rows.
+__device__ __forceinline__ int group_tiles(const DenseArgs& a, int g) {
+  int s0, s1;
+  seq_rows(a, g, s0, s1);
+  return (int)(((int64_t)(s1 - s0) * a.g + kDenseRows - 1) / kDenseRows);
+}
+__device__ __forceinline__ int group_units(const DenseArgs& a, int g, int tk) {
+  return max(1, (shared_of(a, g) + tk - 1) / tk);
+}
+struct GroupPlace { int per, g, base; };
+
+__device__ __forceinline__ GroupPlace group_place(const DenseArgs& a, int wg, int launched, int tk,
+                                                  int32_t* place) {
+  __shared__ int s_tmp[4], s_at[2];
+  auto units = [&](int g) {
+    return g < a.ngroups ? group_tiles(a, g) * group_units(a, g, tk) : 0;
+  };
+  int per = 0;
+  for (int g0 = 0; g0 < a.ngroups; g0 += 256) {
+    const int g = g0 + (int)threadIdx.x;
+    int sum;
+    __syncthreads();
+    const int before = per + block_excl_scan1(units(g), s_tmp, &sum);
+    if (wg == 0 && g < a.ngroups) place[g] = before;
+    per += sum;
+  }
+  if (wg == 0 && threadIdx.x == 0) place[a.ngroups] = per;
+  const Deal deal(per * a.hkv, launched);
+  if ((uint32_t)wg >= deal.grid) return GroupPlace{per, 0, 0};
+  const int u = deal.at(wg) % per;
+  int base = 0;
+  for (int g0 = 0; g0 < a.ngroups; g0 += 256) {
+    const int g = g0 + (int)threadIdx.x, c = units(g);
+    int sum;
+    __syncthreads();
+    const int before = base + block_excl_scan1(c, s_tmp, &sum);
+    if (u >= before && u < before + c) {
+      s_at[0] = g;
+      s_at[1] = before;
+    }
+    base += sum;
+  }
+  __syncthreads();
+  return GroupPlace{per, __builtin_amdgcn_readfirstlane(s_at[0]),
+                    __builtin_amdgcn_readfirstlane(s_at[1])};
+}
+
+// Where a whole tile of a group keeps its part: distinct for all tiles of
+// groups that do not overlap.
+__device__ __forceinline__ int64_t group_slot(const DenseArgs& a, int kvh, int g, int s0, int tile,
+                                              int limit) {
+  return (int64_t)kvh * limit + (int64_t)s0 * a.g / kDenseRows + g + tile;
+}
+
+// The work of one workgroup (wg of nwg).  DIRECT: a tile each, finished here.
+// LISTED: a run of the units of k_plan's tiles.  GROUPED: a run of the units of the
+// groups' shared blocks, parts only.
+enum PrefillKind { DIRECT, LISTED, GROUPED };
+template <int D> constexpr size_t kPrefillLds = 4 * sizeof(uint16_t) * kTk<D> * D;
+
+template <typename T, int D, int MODE, int KIND>
+__device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, const Parts& split,
+                                        const Parts& whole, char* lds, int wg, int nwg) {
   constexpr int TK = kTk<D>;
   constexpr int KB = TK / 32;           // 32-key blocks of S
   constexpr int KS = D / 16;            // QK steps
@@ -170,7 +233,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
   constexpr int KN = TK / RP;           // load instructions per unit and thread
   constexpr int GR = TK / 16;           // runs of 16 keys per unit
   constexpr uint16_t EXPO = __is_same(T, bf16s) ? 0x7f80 : 0x7c00;
-  __shared__ __attribute__((aligned(16))) uint16_t s_k[2][TK * D], s_v[2][TK * D];
+  uint16_t* const s_k = reinterpret_cast<uint16_t*>(lds);         // [2][TK * D]
+  uint16_t* const s_v = s_k + 2 * TK * D;                         // [2][TK * D]
   __shared__ int s_bad, s_range[4][4];
   const int tid = threadIdx.x, lane = lane_id();
   const int w = __builtin_amdgcn_readfirstlane(wave_id());
@@ -181,26 +245,35 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
     const int f0 = min(max(a.starts[0], 0), a.t);
     const int f1 = max(f0, min(max(a.starts[a.requests], 0), a.t));
     const int64_t wide = (int64_t)a.hq * D / 8;
-    for (int t = (int)blockIdx.x; t < f0 + (a.t - f1); t += (int)gridDim.x) {
+    for (int t = wg; t < f0 + (a.t - f1); t += nwg) {
       uint16_t* o = a.out + (int64_t)(t < f0 ? t : f1 + t - f0) * a.hq * D;
       for (int64_t x = tid; x < wide; x += 256) *reinterpret_cast<u16x8*>(o + 8 * x) = u16x8{};
     }
   }
 
-  int u = 0, u1 = 1, kvh, it = 0, per = 0, ntiles = 0, dseq = 0, dtile = 0;
-  if (direct) {
-    const TilePlace at = tile_place(a, (int)blockIdx.x);
-    if (at.kvh >= a.hkv) return;
-    kvh = at.kvh;
-    dseq = at.seq;
-    dtile = at.tile;
+  int u = 0, u1 = 1, kvh, it = 0, per = 0, ntiles = 0, gbase = 0;
+  TilePlace mine{0, 0, 0};
+  if constexpr (KIND == DIRECT) {
+    mine = tile_place(a, wg, nwg);
+    if (mine.kvh >= a.hkv) return;
+    kvh = mine.kvh;
+  } else if constexpr (KIND == GROUPED) {
+    const GroupPlace at = group_place(a, wg, nwg, TK, pl.base);
+    per = at.per;
+    it = at.g;
+    gbase = at.base;
+    const Deal deal(per * a.hkv, nwg);
+    if ((uint32_t)wg >= deal.grid) return;
+    u = deal.at(wg);
+    u1 = deal.at(wg + 1);
+    kvh = u / per;
   } else {
     per = pl.head[0];
     ntiles = pl.head[1];
-    const Deal deal(per * a.hkv, (int)gridDim.x);
-    if (blockIdx.x >= deal.grid) return;
-    u = deal.at((int)blockIdx.x);
-    u1 = deal.at((int)blockIdx.x + 1);
+    const Deal deal(per * a.hkv, nwg);
+    if ((uint32_t)wg >= deal.grid) return;
+    u = deal.at(wg);
+    u1 = deal.at(wg + 1);
     kvh = u / per;
     const int rem = u - kvh * per;
     int lo = 0, hi = ntiles - 1;
@@ -234,8 +307,27 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
   }
 
   while (u < u1) {
-    Tile tl{dseq, dtile, 0, 0, 0, 0, 0, 0};
-    if (!direct) tl = pl.tiles[it];
+    Tile tl{mine.seq, mine.tile, 0, 0, 0, 0, 0, 0};
+    int units = 0;
+    if constexpr (KIND == LISTED) tl = pl.tiles[it];
+    if constexpr (KIND == GROUPED) {
+      if (u == (kvh + 1) * per) {                     // the next KV head's first group
+        ++kvh;
+        it = 0;
+        gbase = 0;
+      }
+      const int rem = u - kvh * per;
+      for (;;) {
+        units = __builtin_amdgcn_readfirstlane(group_units(a, it, TK));
+        const int all = units * __builtin_amdgcn_readfirstlane(group_tiles(a, it));
+        if (rem < gbase + all || it + 1 >= a.ngroups) break;
+        gbase += all;
+        ++it;
+      }
+      tl.seq = it;
+      tl.tile = (rem - gbase) / units;
+      tl.cum = gbase + tl.tile * units;
+    }
     const int seq = __builtin_amdgcn_readfirstlane(tl.seq);
     const int tile = __builtin_amdgcn_readfirstlane(tl.tile);
     int s0, s1;
@@ -258,7 +350,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
     }
     wlo = __builtin_amdgcn_readfirstlane(wlo);
     whi = __builtin_amdgcn_readfirstlane(whi);
-    if (direct) {
+    if constexpr (KIND != LISTED) {
       // the tile's range from its rows, as k_plan lists it
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -271,26 +363,29 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
         s_range[w][2] = mlo;
         s_range[w][3] = mhi;
       }
-      __syncthreads();
+      __syncthreads();                                // (rewritten only after the units' barriers)
       tl.klo = min(min(s_range[0][0], s_range[1][0]), min(s_range[2][0], s_range[3][0]));
       tl.khi = max(max(s_range[0][1], s_range[1][1]), max(s_range[2][1], s_range[3][1]));
       tl.max_lo = max(max(s_range[0][2], s_range[1][2]), max(s_range[2][2], s_range[3][2]));
       tl.min_hi = min(min(s_range[0][3], s_range[1][3]), min(s_range[2][3], s_range[3][3]));
       if (tl.khi <= tl.klo) tl.klo = tl.khi = 0;
-      tl.kstart = tl.klo & ~15;
+      if constexpr (KIND == DIRECT) tl.kstart = tl.klo & ~15;
     }
     const int kstart = __builtin_amdgcn_readfirstlane(tl.kstart);
     const int klo = __builtin_amdgcn_readfirstlane(tl.klo);
     const int khi = __builtin_amdgcn_readfirstlane(tl.khi);
     const int max_lo = __builtin_amdgcn_readfirstlane(tl.max_lo);
     const int min_hi = __builtin_amdgcn_readfirstlane(tl.min_hi);
-    const int n = max(1, (khi - kstart + TK - 1) / TK);
+    const int n = KIND == GROUPED ? units : max(1, (khi - kstart + TK - 1) / TK);
     int j0 = 0, j1 = n;
-    if (!direct) {
+    if constexpr (KIND != DIRECT) {
       j0 = u - (kvh * per + __builtin_amdgcn_readfirstlane(tl.cum));
       j1 = min(n, j0 + (u1 - u));
     }
-    u += direct ? 1 : j1 - j0;
+    u += KIND == DIRECT ? 1 : j1 - j0;
+    // units that some row sees (of a group's shared blocks, windows may hide most)
+    const int ja = KIND == GROUPED ? max(j0, klo / TK) : j0;
+    const int jb = KIND == GROUPED ? min(j1, (khi + TK - 1) / TK) : j1;
     u16x8 qf[KS];
     const uint16_t* qp = a.q + (int64_t)tok * a.qs + (int64_t)head * D + 8 * h;
 #pragma unroll
@@ -298,9 +393,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
     float slope = 0.f;
     if constexpr (MODE & 2) slope = a.slopes[head] * 1.44269504f;
     const int32_t* row =
-        a.table + ((int64_t)(a.groups ? min(max(s0, 0), a.requests - 1) : seq) * a.hkv + kvh) * a.nb;
-    const int kbase = kstart + j0 * TK, kend = min(kstart + j1 * TK, khi);
-    const int cnt = j1 - j0;
+        a.table + ((int64_t)(KIND == GROUPED ? s0 : seq) * a.hkv + kvh) * a.nb;
+    const int kbase = kstart + ja * TK, kend = min(kstart + jb * TK, khi);
+    const int cnt = jb - ja;
 
     auto window = [&](int i) {                        // rows of 64 runs of 16 keys
       const int key = kbase + 16 * (64 * i + lane);
@@ -330,8 +425,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
         if (D == 64 && w >= 2) x = rows[D == 64 ? 2 * i + 1 : 0];
         const int64_t at = (int64_t)max(x, 0) * D + (i * RP % 16) * D;
         const uint32_t slot = (uint32_t)(256 * i + 64 * w) * 16;
-        copy_to_lds(lds_address(s_k[buf]) + slot, a.kp + at, ko[i * RP % 16 ? 1 : 0]);
-        copy_to_lds(lds_address(s_v[buf]) + slot, a.vp + at, vo);
+        copy_to_lds(lds_address(s_k + buf * (TK * D)) + slot, a.kp + at, ko[i * RP % 16 ? 1 : 0]);
+        copy_to_lds(lds_address(s_v + buf * (TK * D)) + slot, a.vp + at, vo);
       }
     };
     // whether some row of the tile does not see all of the unit
@@ -421,7 +516,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
     };
 
     __syncthreads();                                  // the last item's LDS reads are done
-    issue(0, 0);
+    if (KIND != GROUPED || cnt > 0) issue(0, 0);
     bool bad = false;                                 // some rows must skip a value
     for (int j = 0; j < cnt && !bad; ++j) {
       const int buf = j & 1, key0 = kbase + j * TK;
@@ -432,14 +527,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
       __syncthreads();
       if (j + 1 < cnt) issue(j + 1, buf ^ 1);
       if (edge) {
-        clean(key0, mask, s_v[buf]);
+        clean(key0, mask, s_v + buf * (TK * D));
         __syncthreads();
         bad = s_bad == serial;
       }
       if (!bad && key0 < whi && key0 + TK > wlo) {
         u16x8 pf[TK / 16];
-        weights(s_k[buf], key0, edge, mask, pf);
-        const uint16_t* lv = s_v[buf];
+        weights(s_k + buf * (TK * D), key0, edge, mask, pf);
+        const uint16_t* lv = s_v + buf * (TK * D);
 #pragma unroll
         for (int x = 0; x < TK / 16; ++x)
 #pragma unroll
@@ -452,17 +547,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
       }
     }
     const bool all = j0 == 0 && j1 == n;
+    const bool keep = KIND == DIRECT || (KIND == LISTED && all);    // finished here
+    const Parts& to = all ? whole : split;
+    const int64_t slot = all ? group_slot(a, kvh, seq, s0, tile, pl.limit)
+                             : 2 * (int64_t)wg + (j0 > 0 ? 0 : 1);
     if (bad) {
       copies_done();
       __syncthreads();
-      const int64_t slot = all ? (int64_t)kvh * ntiles + it
-                               : 2 * (int64_t)blockIdx.x + (j0 > 0 ? 0 : 1);
       slow_rows<T, D, MODE>(a, seq, s0, s1, (int64_t)tile * kDenseRows + 32 * w, kvh, row, kbase,
-                            kend, all ? whole : split, slot * kDenseRows + 32 * w);
+                            kend, keep ? nullptr : &to, slot * kDenseRows + 32 * w);
     }
     l += __shfl_xor(l, 32);
     if (valid && !bad) {
-      if (all && !whole.m) {
+      if (keep) {
         uint16_t* o = a.out + ((int64_t)tok * a.hq + head) * D + 4 * h;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
@@ -472,9 +569,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
                          f32x4{acc[db][4 * x], acc[db][4 * x + 1], acc[db][4 * x + 2],
                                acc[db][4 * x + 3]}, l);
       } else {
-        const Parts& to = all ? whole : split;
-        const int64_t slot = all ? (int64_t)kvh * ntiles + it
-                                 : 2 * (int64_t)blockIdx.x + (j0 > 0 ? 0 : 1);
         const int64_t pr = slot * kDenseRows + 32 * w + n32;
         float* o = to.o + pr * D + 4 * h;
 #pragma unroll
@@ -489,11 +583,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, 
         }
       }
     }
-    if (++it == ntiles) {
-      it = 0;
-      ++kvh;
-    }
+    if constexpr (KIND == LISTED)
+      if (++it == ntiles) {
+        it = 0;
+        ++kvh;
+      }
   }
+}
+
+template <typename T, int D, int MODE, int KIND>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, Plan pl,
+                                                                   Parts split) {
+  __shared__ __attribute__((aligned(16))) char lds[kPrefillLds<D>];
+  prefill<T, D, MODE, KIND>(a, pl, split, split, lds, (int)blockIdx.x, (int)gridDim.x);
 }
 
 }  // namespace stk

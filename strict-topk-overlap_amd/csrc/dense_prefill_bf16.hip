@@ -1,21 +1,17 @@
-// Dense attention of many query rows, BF16 (dense_prefill.hpp).
+// Dense attention of many rows, BF16 (k_prefill).
 #include "dense_prefill.hpp"
 
 namespace stk {
 
 template <>
 int launch_prefill<bf16s>(int d, int mode, const DenseArgs& a, const Plan& p, const Parts& split,
-                          const Parts& whole, int grid, bool direct, hipStream_t st) {
-#define STK_MODE(D)                                                                              \
-  switch (mode) {                                                                                \
-    case 0: hipLaunchKernelGGL((k_prefill<bf16s, D, 0>), dim3(grid), dim3(256), 0, st, a, p,      \
-                               split, whole, direct); break;                                     \
-    case 1: hipLaunchKernelGGL((k_prefill<bf16s, D, 1>), dim3(grid), dim3(256), 0, st, a, p,      \
-                               split, whole, direct); break;                                     \
-    case 2: hipLaunchKernelGGL((k_prefill<bf16s, D, 2>), dim3(grid), dim3(256), 0, st, a, p,      \
-                               split, whole, direct); break;                                     \
-    default: hipLaunchKernelGGL((k_prefill<bf16s, D, 3>), dim3(grid), dim3(256), 0, st, a, p,     \
-                                split, whole, direct);                                           \
+                       int grid, hipStream_t st) {
+#define STK_MODE(D)                                                                     \
+  switch (mode) {                                                                       \
+    case 0: k_prefill<bf16s, D, 0, LISTED><<<grid, 256, 0, st>>>(a, p, split); break;   \
+    case 1: k_prefill<bf16s, D, 1, LISTED><<<grid, 256, 0, st>>>(a, p, split); break;   \
+    case 2: k_prefill<bf16s, D, 2, LISTED><<<grid, 256, 0, st>>>(a, p, split); break;   \
+    default: k_prefill<bf16s, D, 3, LISTED><<<grid, 256, 0, st>>>(a, p, split); break;  \
   }
   if (d == 64) {
     STK_MODE(64)

@@ -6,16 +6,28 @@ namespace stk {
 
 constexpr int kPlanThreads = 1024;
 
+// A tile of up to kWhole units is not worth cutting.  Cut tiles leave parts that
+// k_join_tiles has to read (64 KB per cut at D = 128) and each workgroup begins
+// twice: about 20 us in all; whole ones leave the device half idle while the
+// longest one ends, about 0.6 us per unit of it.  Causal prompts, 32 query
+// heads over 8 KV heads, D = 128: 1024 tokens 54 us cut, 30 whole; 2048 tokens
+// (longest tile 32 units) 95 cut, 71 whole; but 600 tokens at the end of 12000
+// (188 units each) 80 cut, 118 whole.
+constexpr int kWhole = 40;
+// Cut tiles are dealt in runs of at least kRun units.
+constexpr int kRun = 4;
+
 // Lists the row tiles: one workgroup.  Within a sequence the last rows, which see
-// the most keys, come first.
-__global__ __launch_bounds__(kPlanThreads) void k_plan(DenseArgs a, Plan pl, int tk) {
-  __shared__ int s_a[kPlanThreads / STK_WAVE];
-  const int tid = threadIdx.x, ns = sequences(a);
+// the most keys, come first.  fill: workgroups that fill the device.
+__global__ __launch_bounds__(kPlanThreads) void k_plan(DenseArgs a, Plan pl, int tk, int fill) {
+  __shared__ int s_a[kPlanThreads / STK_WAVE], s_long;
+  const int tid = threadIdx.x, ns = a.requests;
+  if (tid == 0) s_long = 0;
   int base = 0;
   for (int q0 = 0; q0 < ns; q0 += kPlanThreads) {
     const int q = q0 + tid;
     int s0 = 0, s1 = 0, sum;
-    if (q < ns) seq_rows(a, q, s0, s1);
+    if (q < ns) rows_of(a, q, s0, s1);
     const int rt = (int)(((int64_t)(s1 - s0) * a.g + kDenseRows - 1) / kDenseRows);
     __syncthreads();
     const int before = base + block_excl_scan1(rt, s_a, &sum);
@@ -24,58 +36,63 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(DenseArgs a, Plan pl, int
   }
   if (tid == 0) pl.base[ns] = base;
   __syncthreads();                       // the workgroup's own stores are read back
-  const int rt = min(base, pl.limit);
-  int cum = 0;
-  for (int i0 = 0; i0 < rt; i0 += kPlanThreads) {
-    const int i = i0 + tid;
-    Tile x{};
-    int n = 0, sum;
-    if (i < rt) {
-      int lo = 0, hi = ns - 1;           // last sequence that begins at or before tile i
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (pl.base[mid] <= i) lo = mid;
-        else hi = mid - 1;
-      }
-      int s0, s1;
-      seq_rows(a, lo, s0, s1);
-      x.seq = lo;
-      x.tile = pl.base[lo + 1] - 1 - i;
-      const int64_t row0 = (int64_t)x.tile * kDenseRows;
-      const int64_t row1 = min(row0 + kDenseRows, (int64_t)(s1 - s0) * a.g) - 1;
-      const int t0 = s0 + (int)(row0 / a.g), t1 = s0 + (int)(row1 / a.g);
-      x.klo = 0x7fffffff;
-      x.khi = 0;
-      x.max_lo = 0;
-      x.min_hi = 0x7fffffff;
-      // without per-token starts the spans of a request's tokens only move up
-      const int step = a.groups || a.first ? 1 : max(1, t1 - t0);
-      for (int t = t0; t <= t1; t += step) {
-        int p;
-        const Span s = seq_span(a, lo, s0, s1, t, p);
-        if (s.hi > s.lo) {
-          x.klo = min(x.klo, s.lo);
-          x.khi = max(x.khi, s.hi);
-          x.max_lo = max(x.max_lo, s.lo);
-          x.min_hi = min(x.min_hi, s.hi);
-        } else {
-          x.min_hi = 0;
-          // rows after this one may still see keys from their own lower end on
-          if (step > 1) x.klo = min(x.klo, s.lo);
-        }
-      }
-      if (x.khi <= x.klo) x.klo = x.khi = 0;
-      x.kstart = x.klo & ~15;
-      n = max(1, (x.khi - x.kstart + tk - 1) / tk);
+  const int rt = min(min(base, pl.limit), kPlanThreads);
+  // (the host lists no more than kPlanThreads tiles)
+  Tile x{};
+  int n = 0, cum;
+  if (tid < rt) {
+    int lo = 0, hi = ns - 1;             // last sequence that begins at or before this tile
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (pl.base[mid] <= tid) lo = mid;
+      else hi = mid - 1;
     }
-    __syncthreads();
-    x.cum = cum + block_excl_scan1(n, s_a, &sum);
-    if (i < rt) pl.tiles[i] = x;
-    cum += sum;
+    int s0, s1;
+    rows_of(a, lo, s0, s1);
+    x.seq = lo;
+    x.tile = pl.base[lo + 1] - 1 - tid;
+    x.s0 = s0;
+    x.rows = s1 - s0;
+    x.len = tokens_of(a, lo);
+    const int64_t row0 = (int64_t)x.tile * kDenseRows;
+    const int64_t row1 = min(row0 + kDenseRows, (int64_t)x.rows * a.g) - 1;
+    const int t0 = s0 + (int)(row0 / a.g), t1 = s0 + (int)(row1 / a.g);
+    const int p0 = x.len - x.rows - s0;  // position of row t: p0 + t
+    x.klo = 0x7fffffff;
+    x.min_hi = 0x7fffffff;
+    // without per-token starts the spans of a request's tokens only move up
+    const int step = a.first ? 1 : max(1, t1 - t0);
+#pragma unroll 8
+    for (int t = t0; t <= t1; t += step) {
+      const Span s = span_of(a, lo, t, p0 + t, x.len);
+      const bool some = s.hi > s.lo;
+      // without starts rows after an empty one may still see keys from its lower end on
+      x.klo = some || step > 1 ? min(x.klo, s.lo) : x.klo;
+      x.khi = some ? max(x.khi, s.hi) : x.khi;
+      x.max_lo = some ? max(x.max_lo, s.lo) : x.max_lo;
+      x.min_hi = some ? min(x.min_hi, s.hi) : 0;
+    }
+    if (x.khi <= x.klo) x.klo = x.khi = 0;
+    x.kstart = x.klo & ~15;
+    n = max(1, (x.khi - x.kstart + tk - 1) / tk);
+    atomicMax(&s_long, n);
   }
+  __syncthreads();
+  x.cum = block_excl_scan1(n, s_a, &cum);
+  const int most = s_long;
+  int at = tid;
+  if (most <= kWhole) {
+    // whole tiles: the longer half first, so that none of them begins last
+    int first;
+    __syncthreads();
+    const int before = block_excl_scan1(2 * n > most, s_a, &first);
+    at = 2 * n > most ? before : first + tid - before;
+  }
+  if (tid < rt) pl.tiles[at] = x;
   if (tid == 0) {
     pl.head[0] = cum;
     pl.head[1] = rt;
+    pl.head[2] = most <= kWhole ? 0 : min(fill, max(1, cum * a.hkv / kRun));
   }
 }
 
@@ -83,21 +100,21 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(DenseArgs a, Plan pl, int
 // them per workgroup.
 constexpr int kJoinRows = 16;
 template <typename T, int D>
-__global__ __launch_bounds__(256) void k_join_tiles(DenseArgs a, Plan pl, Parts split,
-                                                    int launched) {
+__global__ __launch_bounds__(256) void k_join_tiles(DenseArgs a, Plan pl, Parts split) {
   constexpr int SL = kDenseRows / kJoinRows;
   const int per = pl.head[0], ntiles = pl.head[1];
   const int kvh = (int)blockIdx.x / (pl.limit * SL), x0 = (int)blockIdx.x % (pl.limit * SL);
   const int it = x0 / SL, r0 = (x0 % SL) * kJoinRows;
   if (it >= ntiles) return;
+  if (pl.head[2] == 0) return;
   const Tile t = pl.tiles[it];
   const int first = kvh * per + t.cum;
   const int n = (it + 1 < ntiles ? pl.tiles[it + 1].cum : per) - t.cum;
-  const Deal deal(per * a.hkv, launched);
+  const Deal deal(per * a.hkv, pl.head[2]);
   const int w0 = deal.wg_of(first), w1 = deal.wg_of(first + n - 1);
   if (w0 == w1) return;
   int s0, s1;
-  seq_rows(a, t.seq, s0, s1);
+  rows_of(a, t.seq, s0, s1);
   const int64_t row0 = (int64_t)t.tile * kDenseRows + r0;
   const int nrow = (int)min((int64_t)kJoinRows, (int64_t)(s1 - s0) * a.g - row0);
 #pragma unroll 2
@@ -266,17 +283,21 @@ static int64_t most_units(const DenseShape& s) {
 // Tiles that fill the device several times over need no splitting, and neither do
 // those of caches that hold few units: without it there is nothing to list and
 // nothing to join.
-constexpr int64_t kDirectTiles = 4 * kFill, kDirectUnits = 8;
+constexpr int64_t kDirectTiles = 2 * kFill, kDirectUnits = 8;
 static bool prefill_direct(const DenseShape& s) {
   const int tk = s.d == 256 ? 32 : 64;
   return !s.ngroups && (tile_limit(s) * s.hkv >= kDirectTiles ||
                         (int64_t)s.nb * s.b <= kDirectUnits * tk);
 }
-static int prefill_grid(const DenseShape& s) {
-  if (prefill_direct(s)) return (int)(tile_limit(s) * s.hkv);
-  const int fill = s.d == 256 ? kFill / 2 : kFill;
+static int prefill_fill(const DenseShape& s) {
   const int64_t u = prefill_units(s);
-  return u < fill ? (int)u : fill;
+  return u < kFill ? (int)u : kFill;
+}
+// k_plan decides whether the tiles are cut: there are workgroups for both.
+static int prefill_grid(const DenseShape& s) {
+  const int64_t tiles = tile_limit(s) * s.hkv;
+  const int fill = prefill_fill(s);
+  return s.ngroups || (tiles < fill && !prefill_direct(s)) ? fill : (int)tiles;
 }
 
 static size_t parts_bytes(int64_t slots, int rows, int d) {
@@ -293,13 +314,13 @@ static Parts take_parts(Carve& c, int64_t slots, int rows, int d) {
 // With groups there is no list of tiles: only the units before each group are kept.
 static size_t plan_bytes(const DenseShape& s) {
   if (s.ngroups) return stk_align((s.ngroups + 1) * sizeof(int32_t));
-  return stk_align(2 * sizeof(int32_t)) + stk_align((s.requests + 1) * sizeof(int32_t)) +
+  return stk_align(3 * sizeof(int32_t)) + stk_align((s.requests + 1) * sizeof(int32_t)) +
          stk_align((size_t)tile_limit(s) * sizeof(Tile));
 }
 static Plan take_plan(Carve& c, const DenseShape& s) {
   Plan p{};
   p.limit = (int)tile_limit(s);
-  if (!s.ngroups) p.head = c.take<int32_t>(2);
+  if (!s.ngroups) p.head = c.take<int32_t>(3);
   p.base = c.take<int32_t>((s.ngroups ? s.ngroups : s.requests) + 1);
   if (!s.ngroups) p.tiles = c.take<Tile>(p.limit);
   return p;
@@ -315,25 +336,24 @@ static size_t dense_bytes(const DenseShape& s) {
   }
   if (s.ragged || s.ngroups) {
     if (!prefill_direct(s))
-      x += plan_bytes(s) + parts_bytes(2 * (int64_t)prefill_grid(s), kDenseRows, s.d);
+      x += plan_bytes(s) + parts_bytes(2 * (int64_t)prefill_fill(s), kDenseRows, s.d);
     if (s.ngroups) x += parts_bytes(tile_limit(s) * s.hkv, kDenseRows, s.d);
   }
   return x ? x : 256;
 }
 
-static int launch_plan(const DenseArgs& a, const Plan& p, int d, hipStream_t st) {
-  hipLaunchKernelGGL(k_plan, dim3(1), dim3(kPlanThreads), 0, st, a, p, d == 256 ? 32 : 64);
+static int launch_plan(const DenseArgs& a, const Plan& p, int d, int fill, hipStream_t st) {
+  hipLaunchKernelGGL(k_plan, dim3(1), dim3(kPlanThreads), 0, st, a, p, d == 256 ? 32 : 64, fill);
   return stk_check_launch("k_plan");
 }
 
 template <typename T>
-static void launch_join_tiles(const DenseArgs& a, const Plan& p, const Parts& split, int grid,
-                              int d, hipStream_t st) {
-  const dim3 g((unsigned)(p.limit * a.hkv * (kDenseRows / kJoinRows)));
-  if (d == 64) hipLaunchKernelGGL((k_join_tiles<T, 64>), g, dim3(256), 0, st, a, p, split, grid);
-  else if (d == 128)
-    hipLaunchKernelGGL((k_join_tiles<T, 128>), g, dim3(256), 0, st, a, p, split, grid);
-  else hipLaunchKernelGGL((k_join_tiles<T, 256>), g, dim3(256), 0, st, a, p, split, grid);
+static void launch_join_tiles(const DenseArgs& a, const Plan& p, const Parts& split, int d,
+                              hipStream_t st) {
+  const unsigned g = (unsigned)(p.limit * a.hkv * (kDenseRows / kJoinRows));
+  if (d == 64) k_join_tiles<T, 64><<<g, 256, 0, st>>>(a, p, split);
+  else if (d == 128) k_join_tiles<T, 128><<<g, 256, 0, st>>>(a, p, split);
+  else k_join_tiles<T, 256><<<g, 256, 0, st>>>(a, p, split);
 }
 
 template <typename T, bool SHARED>
@@ -356,12 +376,13 @@ static int run_dense(const DenseShape& s, DenseArgs a, int mode, void* workspace
     const int grid = prefill_grid(s);
     if (prefill_direct(s)) return launch_direct<T>(s.d, mode, a, grid, st);
     const Plan p = take_plan(c, s);
-    const Parts split = take_parts(c, 2 * (int64_t)grid, kDenseRows, s.d);
-    int rc = launch_plan(a, p, s.d, st);
+    const int fill = prefill_fill(s);
+    const Parts split = take_parts(c, 2 * (int64_t)fill, kDenseRows, s.d);
+    int rc = launch_plan(a, p, s.d, fill, st);
     if (rc) return rc;
     rc = launch_prefill<T>(s.d, mode, a, p, split, grid, st);
     if (rc) return rc;
-    launch_join_tiles<T>(a, p, split, grid, s.d, st);
+    launch_join_tiles<T>(a, p, split, s.d, st);
     return stk_check_launch("k_join_tiles");
   }
   const int nc = (a.g + kDecodeRows - 1) / kDecodeRows;
@@ -371,7 +392,7 @@ static int run_dense(const DenseShape& s, DenseArgs a, int mode, void* workspace
   if (s.ngroups) {
     const Parts whole = take_parts(c, (int64_t)s.requests * s.hkv * nc, kDecodeRows, s.d);
     const Plan p = take_plan(c, s);
-    const int pgrid = prefill_grid(s);
+    const int pgrid = prefill_fill(s);
     const Parts ps = take_parts(c, 2 * (int64_t)pgrid, kDenseRows, s.d);
     const Parts pw = take_parts(c, tile_limit(s) * s.hkv, kDenseRows, s.d);
     const int rc = launch_shared<T>(s.d, mode, a, p, ps, pw, pgrid, split, whole, place, grid, st);

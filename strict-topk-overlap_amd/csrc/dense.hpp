@@ -195,12 +195,13 @@ struct Deal {
 };
 
 // Row tiles of the attention of many rows (dense_prefill.hpp), listed on the
-// device: tile `tile` of sequence `seq` reads units of keys from kstart on,
-// `cum` units come before it (per KV head); its rows' keys lie in [klo, khi),
-// and every row sees [max_lo, min_hi).
-struct Tile { int seq, tile, kstart, cum, klo, khi, max_lo, min_hi; };
+// device: tile `tile` of sequence `seq` (query rows s0 .. s0 + rows - 1 of a
+// request of len tokens) reads units of keys from kstart on, `cum` units come
+// before it (per KV head); its rows' keys lie in [klo, khi), and every row sees
+// [max_lo, min_hi).
+struct Tile { int seq, tile, kstart, cum, klo, khi, max_lo, min_hi, s0, rows, len; };
 struct Plan {
-  int32_t* head;      // {units per KV head, tiles}
+  int32_t* head;      // {units per KV head, tiles, workgroups that the units are dealt to (0: tiles are whole)}
   int32_t* base;      // [sequences + 1] first tile of each sequence
   Tile* tiles;
   int limit;          // most tiles there can be

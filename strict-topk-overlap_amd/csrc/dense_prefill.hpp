@@ -44,7 +44,14 @@ __device__ __forceinline__ void copy_to_lds(uint32_t lds, const uint16_t* base, 
                : "s"(lds), "v"(off), "s"(base)
                : "memory");
 }
-__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// The wait is one that the compiler knows: it also settles the queries' and the
+// table's loads, which it would otherwise wait for where they are used, in the
+// middle of every unit, and with them for the copies of the next one.
+__device__ __forceinline__ void copies_done() {
+  asm volatile("" ::: "memory");
+  vm_drain();
+  asm volatile("" ::: "memory");
+}
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
@@ -109,59 +116,44 @@ __device__ void slow_rows(const DenseArgs& a, int seq, int s0, int s1, int64_t r
   }
 }
 
-// The tile of workgroup wg where every tile has its own: tiles of one KV head after
-// the other, dealt to the XCDs in runs, and within a sequence the last rows,
-// which see the most keys, first.  kvh = Hkv: none.
+// The tile of workgroup wg where every tile has its own.  Neighbouring
+// workgroups take one tile of each KV head, so that with eight heads (or a divisor of
+// eight) an XCD, to which every eighth workgroup goes, reads one head's keys;
+// and within a sequence the last rows, which see the most keys, come first.
+// kvh = Hkv: none.
 struct TilePlace { int seq, tile, kvh; };
 
 __device__ __forceinline__ TilePlace tile_place(const DenseArgs& a, int wg, int nwg) {
   __shared__ int s_tmp[4], s_at[2];
-  const int ns = sequences(a);
-  auto tiles = [&](int q) {
-    int s0 = 0, s1 = 0;
-    if (q < ns) seq_rows(a, q, s0, s1);
-    return (int)(((int64_t)(s1 - s0) * a.g + kDenseRows - 1) / kDenseRows);
-  };
-  int total = 0, c0 = 0, b0 = 0, sum0 = 0;
-  for (int q0 = 0; q0 < ns; q0 += 256) {
-    const int c = tiles(q0 + (int)threadIdx.x);
-    int sum;
-    __syncthreads();
-    const int before = block_excl_scan1(c, s_tmp, &sum);   // (of the first 256: from 0)
-    if (q0 == 0) {
-      c0 = c;
-      b0 = before;
-      sum0 = sum;
-    }
-    total += sum;
-  }
-  const int64_t all = min((int64_t)total * a.hkv, (int64_t)nwg);
-  if (wg >= all) return TilePlace{0, 0, a.hkv};
-  const int x = xcd_remap(wg, (int)all), kvh = x / total, it = x % total;
+  const int it = wg / a.hkv;
   int base = 0;
-  for (int q0 = 0; q0 < ns; q0 += 256) {
-    int c = c0, before = b0, sum = sum0;
-    if (q0 > 0) {
-      c = tiles(q0 + (int)threadIdx.x);
-      __syncthreads();
-      before = base + block_excl_scan1(c, s_tmp, &sum);
-    }
+  if (threadIdx.x == 0) s_at[0] = -1;
+  for (int r0 = 0; r0 < a.requests; r0 += 256) {
+    const int r = r0 + (int)threadIdx.x;
+    int s0 = 0, s1 = 0, sum;
+    if (r < a.requests) rows_of(a, r, s0, s1);
+    const int c = (int)(((int64_t)(s1 - s0) * a.g + kDenseRows - 1) / kDenseRows);
+    __syncthreads();
+    const int before = base + block_excl_scan1(c, s_tmp, &sum);
     if (it >= before && it < before + c) {
-      s_at[0] = q0 + (int)threadIdx.x;
+      s_at[0] = r;
       s_at[1] = before + c - 1 - it;
     }
     base += sum;
+    if (it < base) break;
   }
   __syncthreads();
-  return TilePlace{__builtin_amdgcn_readfirstlane(s_at[0]),
-                   __builtin_amdgcn_readfirstlane(s_at[1]), kvh};
+  const int r = __builtin_amdgcn_readfirstlane(s_at[0]);
+  if (r < 0) return TilePlace{0, 0, a.hkv};
+  return TilePlace{r, __builtin_amdgcn_readfirstlane(s_at[1]), wg % a.hkv};
 }
 
 // Shared blocks: every tile of a group has the same units, those of its
 // shared blocks.  The units of the groups' tiles end to end, per KV head: how many
 // there are, the group that holds unit u (taken modulo them), and the units before
-// it.  Workgroup 0 also leaves the units before every group, and their total, in
-// place [groups + 1] for k_join_rows.
+// it.  u is the first unit of workgroup wg, which becomes its place among the
+// workgroups with work.  Workgroup 0 also leaves the units before every group, and
+// their total, in place [groups + 1] for k_join_rows.
 __device__ __forceinline__ int group_tiles(const DenseArgs& a, int g) {
   int s0, s1;
   seq_rows(a, g, s0, s1);
@@ -170,9 +162,9 @@ __device__ __forceinline__ int group_tiles(const DenseArgs& a, int g) {
 __device__ __forceinline__ int group_units(const DenseArgs& a, int g, int tk) {
   return max(1, (shared_of(a, g) + tk - 1) / tk);
 }
-struct GroupPlace { int per, g, base; };
+struct GroupPlace { int per, g, base; };      // per = 0: no work
 
-__device__ __forceinline__ GroupPlace group_place(const DenseArgs& a, int wg, int launched, int tk,
+__device__ __forceinline__ GroupPlace group_place(const DenseArgs& a, int& wg, int launched, int tk,
                                                   int32_t* place) {
   __shared__ int s_tmp[4], s_at[2];
   auto units = [&](int g) {
@@ -189,7 +181,8 @@ __device__ __forceinline__ GroupPlace group_place(const DenseArgs& a, int wg, in
   }
   if (wg == 0 && threadIdx.x == 0) place[a.ngroups] = per;
   const Deal deal(per * a.hkv, launched);
-  if ((uint32_t)wg >= deal.grid) return GroupPlace{per, 0, 0};
+  if ((uint32_t)wg >= deal.grid) return GroupPlace{0, 0, 0};
+  wg = xcd_remap(wg, (int)deal.grid);
   const int u = deal.at(wg) % per;
   int base = 0;
   for (int g0 = 0; g0 < a.ngroups; g0 += 256) {
@@ -215,8 +208,10 @@ __device__ __forceinline__ int64_t group_slot(const DenseArgs& a, int kvh, int g
   return (int64_t)kvh * limit + (int64_t)s0 * a.g / kDenseRows + g + tile;
 }
 
-// The work of one workgroup (wg of nwg).  DIRECT: a tile each, finished here.
-// LISTED: a run of the units of k_plan's tiles.  GROUPED: a run of the units of the
+// The work of one workgroup (wg of nwg).  The runs of neighbouring units, which
+// read the same keys, go to one XCD (one L2).  DIRECT: a tile each, finished here.
+// LISTED: a tile of
+// k_plan's each, or a run of their units.  GROUPED: a run of the units of the
 // groups' shared blocks, parts only.
 enum PrefillKind { DIRECT, LISTED, GROUPED };
 template <int D> constexpr size_t kPrefillLds = 4 * sizeof(uint16_t) * kTk<D> * D;
@@ -232,10 +227,11 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
   constexpr int RP = 256 / CPR;         // rows per load instruction of the workgroup
   constexpr int KN = TK / RP;           // load instructions per unit and thread
   constexpr int GR = TK / 16;           // runs of 16 keys per unit
+  constexpr bool AHEAD = D <= 128;      // operands requested ahead of their use
   constexpr uint16_t EXPO = __is_same(T, bf16s) ? 0x7f80 : 0x7c00;
-  uint16_t* const s_k = reinterpret_cast<uint16_t*>(lds);         // [2][TK * D]
-  uint16_t* const s_v = s_k + 2 * TK * D;                         // [2][TK * D]
-  __shared__ int s_bad, s_range[4][4];
+  constexpr int UNIT = 2 * TK * D;      // bytes of K or V: lds holds K, K, V, V
+  const uint32_t lds_k = lds_address(lds);
+  __shared__ int s_bad[2], s_range[4][4];
   const int tid = threadIdx.x, lane = lane_id();
   const int w = __builtin_amdgcn_readfirstlane(wave_id());
   const int n32 = lane & 31, h = lane >> 5, i16 = lane & 15, gq = (lane >> 4) & 1;
@@ -253,61 +249,69 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
 
   int u = 0, u1 = 1, kvh, it = 0, per = 0, ntiles = 0, gbase = 0;
   TilePlace mine{0, 0, 0};
+  bool whole_tile = KIND == DIRECT;
   if constexpr (KIND == DIRECT) {
     mine = tile_place(a, wg, nwg);
     if (mine.kvh >= a.hkv) return;
     kvh = mine.kvh;
   } else if constexpr (KIND == GROUPED) {
     const GroupPlace at = group_place(a, wg, nwg, TK, pl.base);
+    if (at.per == 0) return;
     per = at.per;
     it = at.g;
     gbase = at.base;
     const Deal deal(per * a.hkv, nwg);
-    if ((uint32_t)wg >= deal.grid) return;
     u = deal.at(wg);
     u1 = deal.at(wg + 1);
     kvh = u / per;
   } else {
     per = pl.head[0];
     ntiles = pl.head[1];
-    const Deal deal(per * a.hkv, nwg);
-    if ((uint32_t)wg >= deal.grid) return;
-    u = deal.at(wg);
-    u1 = deal.at(wg + 1);
-    kvh = u / per;
-    const int rem = u - kvh * per;
-    int lo = 0, hi = ntiles - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (pl.tiles[mid].cum <= rem) lo = mid;
-      else hi = mid - 1;
+    const int cut = pl.head[2];
+    whole_tile = cut == 0;
+    if (whole_tile) {                     // a tile each, dealt as tile_place does
+      if (wg >= ntiles * a.hkv) return;
+      kvh = wg % a.hkv;
+      it = wg / a.hkv;
+    } else {
+      const Deal deal(per * a.hkv, cut);
+      if ((uint32_t)wg >= deal.grid) return;
+      wg = xcd_remap(wg, (int)deal.grid);
+      u = deal.at(wg);
+      u1 = deal.at(wg + 1);
+      kvh = u / per;
+      const int rem = u - kvh * per;
+      int lo = 0, hi = ntiles - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (pl.tiles[mid].cum <= rem) lo = mid;
+        else hi = mid - 1;
+      }
+      it = __builtin_amdgcn_readfirstlane(lo);
     }
-    it = __builtin_amdgcn_readfirstlane(lo);
   }
-  if (tid == 0) s_bad = 0;
+  if (tid < 2) s_bad[tid] = 0;
   int serial = 0;                       // units worked on so far, in this workgroup
 
-  // LDS addresses (elements)
+  // K rows are swizzled in 16-byte chunks, V rows in 64-byte blocks
   auto fk = [](int row) { return D == 64 ? (row >> 1) & 7 : row & 15; };
   auto fv = [](int row) { return D == 64 ? (row >> 1) & 1 : row & 3; };
   const int lrow = tid / CPR, lch = tid % CPR;
-  // byte offsets of this lane's K (for D = 256 of both halves of a run) and V chunk
+  // byte offsets of this lane's K (for D = 256 of both halves of a run) and V
+  // chunk within a run of 16 pool rows
   uint32_t ko[2], vo;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     ko[i] = ((lrow & 15) * D + (lch ^ fk(lrow + (D == 256 ? 8 * i : 0))) * 8) * 2;
   vo = ((lrow & 15) * D + ((((lch >> 2) ^ fv(lrow)) << 2) | (lch & 3)) * 8) * 2;
-  int ka[KS], va[DB];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) ka[s] = n32 * D + ((2 * s + h) ^ fk(n32)) * 8;
-#pragma unroll
-  for (int db = 0; db < DB; ++db) {
-    const int row = 4 * h + (i16 >> 2);
-    va[db] = row * D + (db ^ fv(row)) * 32 + 16 * gq + 4 * (i16 & 3);
-  }
+  // LDS byte offsets of the products' operands at step 0; the others' differ
+  // by an exclusive or, since a row's start is aligned to its size
+  const uint32_t ka = (n32 * D + (h ^ fk(n32)) * 8) * 2;
+  const int vrow = 4 * h + (i16 >> 2);
+  const uint32_t va = (vrow * D + fv(vrow) * 32 + 16 * gq + 4 * (i16 & 3)) * 2;
 
   while (u < u1) {
-    Tile tl{mine.seq, mine.tile, 0, 0, 0, 0, 0, 0};
+    Tile tl{mine.seq, mine.tile, 0, 0, 0, 0, 0, 0, 0, 0, 0};
     int units = 0;
     if constexpr (KIND == LISTED) tl = pl.tiles[it];
     if constexpr (KIND == GROUPED) {
@@ -330,38 +334,46 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
     }
     const int seq = __builtin_amdgcn_readfirstlane(tl.seq);
     const int tile = __builtin_amdgcn_readfirstlane(tl.tile);
-    int s0, s1;
-    seq_rows(a, seq, s0, s1);
+    if constexpr (KIND != LISTED) {
+      int s1;
+      seq_rows(a, seq, tl.s0, s1);
+      tl.rows = s1 - tl.s0;
+      tl.len = KIND == DIRECT ? tokens_of(a, seq) : 0;
+    }
+    const int s0 = __builtin_amdgcn_readfirstlane(tl.s0);
+    const int nrow = __builtin_amdgcn_readfirstlane(tl.rows);
     const int64_t rown = (int64_t)tile * kDenseRows + 32 * w + n32;
-    const bool valid = rown < (int64_t)(s1 - s0) * a.g;
+    const bool valid = rown < (int64_t)nrow * a.g;
     const int tok = s0 + (int)(valid ? rown / a.g : 0);
     const int head = kvh * a.g + (int)(valid ? rown % a.g : 0);
-    int p = 0;
-    Span sp = seq_span(a, seq, s0, s1, tok, p);
-    // keys that some row of this wave sees
-    int wlo = valid && sp.hi > sp.lo ? sp.lo : 0x7fffffff;
-    int whi = valid && sp.hi > sp.lo ? sp.hi : 0;
-    int mlo = valid ? sp.lo : 0, mhi = valid ? (sp.hi > sp.lo ? sp.hi : 0) : 0x7fffffff;
-    if (!valid) sp = Span{0, 0x7fffffff};
+    u16x8 qf[KS];
+    const uint16_t* qp = a.q + (int64_t)tok * a.qs + (int64_t)head * D + 8 * h;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      wlo = min(wlo, __shfl_xor(wlo, o));
-      whi = max(whi, __shfl_xor(whi, o));
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u16x8*>(qp + 16 * s);
+    float slope = 0.f;
+    if constexpr (MODE & 2) slope = a.slopes[head] * 1.44269504f;
+    int p;
+    Span sp;
+    if constexpr (KIND == GROUPED) {
+      sp = seq_span(a, seq, s0, s0 + nrow, tok, p);
+    } else {
+      const int len = __builtin_amdgcn_readfirstlane(tl.len);
+      p = len - nrow + (tok - s0);
+      sp = span_of(a, seq, tok, p, len);
     }
-    wlo = __builtin_amdgcn_readfirstlane(wlo);
-    whi = __builtin_amdgcn_readfirstlane(whi);
+    // keys that some row of this wave sees
+    const bool some = valid && sp.hi > sp.lo;
+    const int wlo = (int)wave_ext_u32<false>(some ? (uint32_t)sp.lo : 0x7fffffffu);
+    const int whi = (int)wave_ext_u32<true>(some ? (uint32_t)sp.hi : 0u);
     if constexpr (KIND != LISTED) {
       // the tile's range from its rows, as k_plan lists it
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        mlo = max(mlo, __shfl_xor(mlo, o));
-        mhi = min(mhi, __shfl_xor(mhi, o));
-      }
+      const uint32_t mlo = wave_ext_u32<true>(some ? (uint32_t)sp.lo : 0u);
+      const uint32_t mhi = wave_ext_u32<false>(valid ? (some ? (uint32_t)sp.hi : 0u) : 0x7fffffffu);
       if (lane == 0) {
         s_range[w][0] = wlo;
         s_range[w][1] = whi;
-        s_range[w][2] = mlo;
-        s_range[w][3] = mhi;
+        s_range[w][2] = (int)mlo;
+        s_range[w][3] = (int)mhi;
       }
       __syncthreads();                                // (rewritten only after the units' barriers)
       tl.klo = min(min(s_range[0][0], s_range[1][0]), min(s_range[2][0], s_range[3][0]));
@@ -378,22 +390,15 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
     const int min_hi = __builtin_amdgcn_readfirstlane(tl.min_hi);
     const int n = KIND == GROUPED ? units : max(1, (khi - kstart + TK - 1) / TK);
     int j0 = 0, j1 = n;
-    if constexpr (KIND != DIRECT) {
+    if (!whole_tile) {
       j0 = u - (kvh * per + __builtin_amdgcn_readfirstlane(tl.cum));
       j1 = min(n, j0 + (u1 - u));
     }
-    u += KIND == DIRECT ? 1 : j1 - j0;
+    u += whole_tile ? 1 : j1 - j0;
     // units that some row sees (of a group's shared blocks, windows may hide most)
     const int ja = KIND == GROUPED ? max(j0, klo / TK) : j0;
     const int jb = KIND == GROUPED ? min(j1, (khi + TK - 1) / TK) : j1;
-    u16x8 qf[KS];
-    const uint16_t* qp = a.q + (int64_t)tok * a.qs + (int64_t)head * D + 8 * h;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u16x8*>(qp + 16 * s);
-    float slope = 0.f;
-    if constexpr (MODE & 2) slope = a.slopes[head] * 1.44269504f;
-    const int32_t* row =
-        a.table + ((int64_t)(KIND == GROUPED ? s0 : seq) * a.hkv + kvh) * a.nb;
+    const int32_t* row = a.table + ((int64_t)(KIND == GROUPED ? s0 : seq) * a.hkv + kvh) * a.nb;
     const int kbase = kstart + ja * TK, kend = min(kstart + jb * TK, khi);
     const int cnt = jb - ja;
 
@@ -402,7 +407,7 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
       const int x = pool_row(a, row, min(key, kend));
       return key < kend ? x : -1;
     };
-    int ent = window(0), nxt = window(1);
+    int ent = window(0), nxt = cnt * GR > 64 ? window(1) : -1;
     int vmask = 0;                                    // runs with a page, of the unit last issued
     // Lane l of wave w fills the 16-byte slot 256 i + 64 w + l of the unit's LDS: row
     // i RP + lrow, and of that row the chunk that the swizzle puts there.  A
@@ -424,27 +429,40 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
         int x = rows[D == 64 ? 2 * i : i * RP / 16];
         if (D == 64 && w >= 2) x = rows[D == 64 ? 2 * i + 1 : 0];
         const int64_t at = (int64_t)max(x, 0) * D + (i * RP % 16) * D;
-        const uint32_t slot = (uint32_t)(256 * i + 64 * w) * 16;
-        copy_to_lds(lds_address(s_k + buf * (TK * D)) + slot, a.kp + at, ko[i * RP % 16 ? 1 : 0]);
-        copy_to_lds(lds_address(s_v + buf * (TK * D)) + slot, a.vp + at, vo);
+        const uint32_t slot = (uint32_t)(buf * UNIT + (256 * i + 64 * w) * 16);
+        copy_to_lds(lds_k + slot, a.kp + at, ko[i * RP % 16 ? 1 : 0]);
+        copy_to_lds(lds_k + 2 * UNIT + slot, a.vp + at, vo);
       }
     };
-    // whether some row of the tile does not see all of the unit
-    auto masked = [&](int key0) {
-      return !(key0 >= max_lo && key0 + TK <= min_hi && vmask == (1 << GR) - 1);
-    };
-    // Values of the unit that no row sees become zero; s_bad = serial if any other
-    // is not finite.
-    auto clean = [&](int key0, int mask, uint16_t* lv) {
+    // A value that a row does not see may be infinite or NaN, and 0 times it is
+    // not 0.  Where no row of the tile sees it, it becomes zero (`cut`); any
+    // other one leaves the unit's serial number in s_bad.
+    auto clean = [&](int key0, int mask, int buf, bool cut) {
       bool bad = false;
 #pragma unroll
       for (int i = 0; i < KN; ++i) {
         const int kr = i * RP + lrow, key = key0 + kr;
-        u16x8* at = reinterpret_cast<u16x8*>(lv + (256 * i + tid) * 8);
-        if (key >= klo && key < khi && (mask >> (kr / 16) & 1)) bad |= nonfinite16(*at, EXPO);
+        u16x8* at = reinterpret_cast<u16x8*>(lds + (2 + buf) * UNIT + (256 * i + tid) * 16);
+        const bool seen = !cut || (key >= klo && key < khi && (mask >> (kr / 16) & 1));
+        if (seen) bad |= nonfinite16(*at, EXPO);
         else *at = u16x8{};
       }
-      if (bad) s_bad = serial;
+      if (bad) s_bad[buf] = serial;
+    };
+
+    // V^T for one step of the second product: 16 keys, 32 dims
+    auto v_part = [&](const char* at) {
+      const u16x4 lo = lds_tr(reinterpret_cast<const uint16_t*>(at));
+      const u16x4 hi = lds_tr(reinterpret_cast<const uint16_t*>(at + 16 * D));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    u16x8 vf[AHEAD ? TK / 16 : 1][DB];
+    auto read_v = [&](int buf) {
+#pragma unroll
+      for (int x = 0; x < (AHEAD ? TK / 16 : 1); ++x)
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          vf[x][db] = v_part(lds + (2 + buf) * UNIT + (va ^ (64 * db)) + 32 * x * D);
     };
 
     float m = -INFINITY, l = 0.f;
@@ -454,18 +472,63 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
 #pragma unroll
       for (int x = 0; x < 16; ++x) acc[i][x] = 0.f;
 
-    // P of the unit whose K is lk, as the second product's operand; m, l and
-    // the output follow its maximum
-    auto weights = [&](const uint16_t* lk, int key0, bool edge, int mask,
-                       u16x8 (&pf)[TK / 16]) {
+    __syncthreads();                                  // the last item's LDS reads are done
+    if (KIND != GROUPED || cnt > 0) issue(0, 0);
+    // some row must skip a value: found one barrier after the unit's check
+    bool bad = false, edge = false;
+    for (int j = 0; j < cnt; ++j) {
+      const int buf = j & 1, key0 = kbase + j * TK, mask = vmask;
+      const bool before = edge;
+      edge = !(key0 >= max_lo && key0 + TK <= min_hi && mask == (1 << GR) - 1);
+      copies_done();
+      __syncthreads();
+      if (before) bad = s_bad[buf ^ 1] == serial;
+      if (bad) break;
+      ++serial;
+      if (j + 1 < cnt) issue(j + 1, buf ^ 1);
+      if (edge) {
+        const bool cut = key0 < klo || key0 + TK > khi || mask != (1 << GR) - 1;
+        clean(key0, mask, buf, cut);
+        if (cut) __syncthreads();
+      }
+      if (key0 >= whi || key0 + TK <= wlo) continue;
+
+      // P^T of the unit; m, l and the output follow its maximum
       f32x16 s[KB];
+      u16x8 pf[TK / 16];
+      {
+        uint32_t kb = ka;
+        if constexpr (D == 256) asm volatile("" : "+v"(kb));   // (keeps 16 offsets out of registers)
+        const char* lk = lds + buf * UNIT;
 #pragma unroll
-      for (int b = 0; b < KB; ++b) {
+        for (int b = 0; b < KB; ++b)
 #pragma unroll
-        for (int x = 0; x < 16; ++x) s[b][x] = 0.f;
+          for (int x = 0; x < 16; ++x) s[b][x] = 0.f;
+        // where registers allow, the unit's K is requested at once and its V before
+        // the softmax: the matrix instructions find their operands
+        if constexpr (AHEAD) {
+          u16x8 kf[KS][KB];
 #pragma unroll
-        for (int x = 0; x < KS; ++x)
-          s[b] = mma32<T>(*reinterpret_cast<const u16x8*>(lk + ka[x] + 32 * b * D), qf[x], s[b]);
+          for (int x = 0; x < KS; ++x)
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+              kf[x][b] = *reinterpret_cast<const u16x8*>(lk + (kb ^ (32 * x)) + 64 * b * D);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int x = 0; x < KS; ++x)
+#pragma unroll
+            for (int b = 0; b < KB; ++b) s[b] = mma32<T>(kf[x][b], qf[x], s[b]);
+          __builtin_amdgcn_sched_barrier(0);
+          read_v(buf);
+          __builtin_amdgcn_sched_barrier(0);
+        } else {
+#pragma unroll
+          for (int x = 0; x < KS; ++x)
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+              s[b] = mma32<T>(
+                  *reinterpret_cast<const u16x8*>(lk + (kb ^ (32 * x)) + 64 * b * D), qf[x], s[b]);
+        }
       }
       // MODE 0 keeps the products as they are: their scale goes into the exponent's FMA
       const float sc = MODE ? 1.f : a.c;
@@ -480,14 +543,21 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
           }
       }
       if (edge) {
+        // key0 + 4 h + off in [lo, hi), as one unsigned comparison
+        const int rlo = sp.lo - key0 - 4 * h;
+        const uint32_t wide = (uint32_t)max(sp.hi - sp.lo, 0);
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const int key = key0 + 4 * h + 32 * b + 8 * (x / 4) + x % 4;
-            const bool ok = key >= sp.lo && key < sp.hi && (mask >> (2 * b + x / 8) & 1);
-            s[b][x] = ok ? s[b][x] : -INFINITY;
-          }
+          for (int x = 0; x < 16; ++x)
+            s[b][x] = (uint32_t)(32 * b + 8 * (x / 4) + x % 4 - rlo) < wide ? s[b][x] : -INFINITY;
+        if (mask != (1 << GR) - 1) {
+#pragma unroll
+          for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+              s[b][x] = mask >> (2 * b + x / 8) & 1 ? s[b][x] : -INFINITY;
+        }
       }
       float top = s[0][0];
 #pragma unroll
@@ -513,38 +583,25 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
           l += e;
           pf[2 * b + x / 8][x % 8] = to16<T>(e);
         }
-    };
-
-    __syncthreads();                                  // the last item's LDS reads are done
-    if (KIND != GROUPED || cnt > 0) issue(0, 0);
-    bool bad = false;                                 // some rows must skip a value
-    for (int j = 0; j < cnt && !bad; ++j) {
-      const int buf = j & 1, key0 = kbase + j * TK;
-      const int mask = vmask;
-      const bool edge = masked(key0);
-      ++serial;
-      copies_done();
-      __syncthreads();
-      if (j + 1 < cnt) issue(j + 1, buf ^ 1);
-      if (edge) {
-        clean(key0, mask, s_v + buf * (TK * D));
-        __syncthreads();
-        bad = s_bad == serial;
-      }
-      if (!bad && key0 < whi && key0 + TK > wlo) {
-        u16x8 pf[TK / 16];
-        weights(s_k + buf * (TK * D), key0, edge, mask, pf);
-        const uint16_t* lv = s_v + buf * (TK * D);
+      if constexpr (AHEAD) {
 #pragma unroll
         for (int x = 0; x < TK / 16; ++x)
 #pragma unroll
-          for (int db = 0; db < DB; ++db) {
-            const u16x4 lo = lds_tr(lv + va[db] + 16 * x * D);
-            const u16x4 hi = lds_tr(lv + va[db] + (16 * x + 8) * D);
-            acc[db] = mma32<T>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pf[x],
-                               acc[db]);
-          }
+          for (int db = 0; db < DB; ++db) acc[db] = mma32<T>(vf[x][db], pf[x], acc[db]);
+      } else {
+        uint32_t vb = va;
+        asm volatile("" : "+v"(vb));
+#pragma unroll
+        for (int x = 0; x < TK / 16; ++x)
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+            acc[db] = mma32<T>(v_part(lds + (2 + buf) * UNIT + (vb ^ (64 * db)) + 32 * x * D),
+                               pf[x], acc[db]);
       }
+    }
+    if (edge && !bad) {                               // the last unit's check
+      __syncthreads();
+      bad = s_bad[(cnt - 1) & 1] == serial;
     }
     const bool all = j0 == 0 && j1 == n;
     const bool keep = KIND == DIRECT || (KIND == LISTED && all);    // finished here
@@ -552,10 +609,8 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
     const int64_t slot = all ? group_slot(a, kvh, seq, s0, tile, pl.limit)
                              : 2 * (int64_t)wg + (j0 > 0 ? 0 : 1);
     if (bad) {
-      copies_done();
-      __syncthreads();
-      slow_rows<T, D, MODE>(a, seq, s0, s1, (int64_t)tile * kDenseRows + 32 * w, kvh, row, kbase,
-                            kend, keep ? nullptr : &to, slot * kDenseRows + 32 * w);
+      slow_rows<T, D, MODE>(a, seq, s0, s0 + nrow, (int64_t)tile * kDenseRows + 32 * w, kvh, row,
+                            kbase, kend, keep ? nullptr : &to, slot * kDenseRows + 32 * w);
     }
     l += __shfl_xor(l, 32);
     if (valid && !bad) {
@@ -592,9 +647,9 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
 }
 
 template <typename T, int D, int MODE, int KIND>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_prefill(DenseArgs a, Plan pl,
+__global__ __launch_bounds__(256, 2) void k_prefill(DenseArgs a, Plan pl,
                                                                    Parts split) {
-  __shared__ __attribute__((aligned(16))) char lds[kPrefillLds<D>];
+  __shared__ __attribute__((aligned(1024))) char lds[kPrefillLds<D>];
   prefill<T, D, MODE, KIND>(a, pl, split, split, lds, (int)blockIdx.x, (int)gridDim.x);
 }
 

@@ -17,7 +17,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_shared(DenseArgs a, P
                                                                   Parts split, Parts whole,
                                                                   int32_t* place) {
   constexpr size_t N = kPrefillLds<D> > kDecodeLds<D> ? kPrefillLds<D> : kDecodeLds<D>;
-  __shared__ __attribute__((aligned(16))) char lds[N];
+  __shared__ __attribute__((aligned(1024))) char lds[N];
   const int wg = (int)blockIdx.x;
   if (wg < pgrid) {
     prefill<T, D, MODE, GROUPED>(a, pl, psplit, pwhole, lds, wg, pgrid);

@@ -4,136 +4,140 @@
 
 namespace stk {
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 1024;     // and the most requests and tiles that are listed
 
 // A tile of up to kWhole units is not worth cutting.  Cut tiles leave parts that
-// k_join_tiles has to read (64 KB per cut at D = 128) and each workgroup begins
-// twice: about 20 us in all; whole ones leave the device half idle while the
-// longest one ends, about 0.6 us per unit of it.  Causal prompts, 32 query
-// heads over 8 KV heads, D = 128: 1024 tokens 54 us cut, 30 whole; 2048 tokens
-// (longest tile 32 units) 95 cut, 71 whole; but 600 tokens at the end of 12000
-// (188 units each) 80 cut, 118 whole.
+// k_join_tiles has to read (64 KB per cut at D = 128), and each workgroup begins
+// twice; whole ones leave part of the device idle while the longest one ends.
+// Causal prompts, 32 query heads over 8 KV heads, D = 128: 1024 tokens 54 us
+// cut, 37 whole; 2048 tokens (longest tile 32 units) 95 cut, 65 whole.
 constexpr int kWhole = 40;
 // Cut tiles are dealt in runs of at least kRun units.
 constexpr int kRun = 4;
 
-// Lists the row tiles: one workgroup.  Within a sequence the last rows, which see
-// the most keys, come first.  fill: workgroups that fill the device.
+// Lists the row tiles: one workgroup.  Within a request the last rows, which see
+// the most keys, come first; whole tiles are listed by their length, the longest
+// first.  fill: workgroups that fill the device.
 __global__ __launch_bounds__(kPlanThreads) void k_plan(DenseArgs a, Plan pl, int tk, int fill) {
-  __shared__ int s_a[kPlanThreads / STK_WAVE], s_long;
+  __shared__ int s_a[kPlanThreads / STK_WAVE], s_b[kPlanThreads / STK_WAVE], s_long;
+  __shared__ int s_base[kPlanThreads + 1], s_s0[kPlanThreads], s_rows[kPlanThreads],
+      s_len[kPlanThreads], s_count[kWhole + 1];
   const int tid = threadIdx.x, ns = a.requests;
   if (tid == 0) s_long = 0;
-  int base = 0;
-  for (int q0 = 0; q0 < ns; q0 += kPlanThreads) {
-    const int q = q0 + tid;
-    int s0 = 0, s1 = 0, sum;
-    if (q < ns) rows_of(a, q, s0, s1);
-    const int rt = (int)(((int64_t)(s1 - s0) * a.g + kDenseRows - 1) / kDenseRows);
-    __syncthreads();
-    const int before = base + block_excl_scan1(rt, s_a, &sum);
-    if (q < ns) pl.base[q] = before;
-    base += sum;
+  if (tid <= kWhole) s_count[tid] = 0;
+  int s0 = 0, s1 = 0, base;
+  if (tid < ns) {
+    rows_of(a, tid, s0, s1);
+    s_s0[tid] = s0;
+    s_rows[tid] = s1 - s0;
+    s_len[tid] = tokens_of(a, tid);
   }
-  if (tid == 0) pl.base[ns] = base;
-  __syncthreads();                       // the workgroup's own stores are read back
+  const int mine = (int)(((int64_t)(s1 - s0) * a.g + kDenseRows - 1) / kDenseRows);
+  s_base[tid] = block_excl_scan1(mine, s_a, &base);
+  __syncthreads();
   const int rt = min(min(base, pl.limit), kPlanThreads);
-  // (the host lists no more than kPlanThreads tiles)
   Tile x{};
   int n = 0, cum;
   if (tid < rt) {
-    int lo = 0, hi = ns - 1;             // last sequence that begins at or before this tile
+    int lo = 0, hi = ns - 1;             // last request that begins at or before this tile
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
-      if (pl.base[mid] <= tid) lo = mid;
+      if (s_base[mid] <= tid) lo = mid;
       else hi = mid - 1;
     }
-    int s0, s1;
-    rows_of(a, lo, s0, s1);
     x.seq = lo;
-    x.tile = pl.base[lo + 1] - 1 - tid;
-    x.s0 = s0;
-    x.rows = s1 - s0;
-    x.len = tokens_of(a, lo);
+    x.tile = (lo + 1 < ns ? s_base[lo + 1] : base) - 1 - tid;
+    x.s0 = s_s0[lo];
+    x.rows = s_rows[lo];
+    x.len = s_len[lo];
     const int64_t row0 = (int64_t)x.tile * kDenseRows;
     const int64_t row1 = min(row0 + kDenseRows, (int64_t)x.rows * a.g) - 1;
-    const int t0 = s0 + (int)(row0 / a.g), t1 = s0 + (int)(row1 / a.g);
-    const int p0 = x.len - x.rows - s0;  // position of row t: p0 + t
+    const int t0 = x.s0 + (int)(row0 / a.g), t1 = x.s0 + (int)(row1 / a.g);
+    const int p0 = x.len - x.rows - x.s0;          // position of row t: p0 + t
     x.klo = 0x7fffffff;
     x.min_hi = 0x7fffffff;
-    // without per-token starts the spans of a request's tokens only move up
-    const int step = a.first ? 1 : max(1, t1 - t0);
-#pragma unroll 8
-    for (int t = t0; t <= t1; t += step) {
-      const Span s = span_of(a, lo, t, p0 + t, x.len);
+    auto see = [&](int t, int first) {
+      const Span s = span_at(a, lo, first, p0 + t, x.len);
       const bool some = s.hi > s.lo;
       // without starts rows after an empty one may still see keys from its lower end on
-      x.klo = some || step > 1 ? min(x.klo, s.lo) : x.klo;
+      x.klo = some || !a.first ? min(x.klo, s.lo) : x.klo;
       x.khi = some ? max(x.khi, s.hi) : x.khi;
       x.max_lo = some ? max(x.max_lo, s.lo) : x.max_lo;
       x.min_hi = some ? min(x.min_hi, s.hi) : 0;
+    };
+    if (a.first) {
+      for (int t = t0; t <= t1; t += 16) {
+        int f[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] = a.first[min(t + i, t1)];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) see(min(t + i, t1), f[i]);
+      }
+    } else {                             // the spans of a request's tokens only move up
+      see(t0, 0);
+      see(t1, 0);
     }
     if (x.khi <= x.klo) x.klo = x.khi = 0;
     x.kstart = x.klo & ~15;
     n = max(1, (x.khi - x.kstart + tk - 1) / tk);
     atomicMax(&s_long, n);
   }
-  __syncthreads();
-  x.cum = block_excl_scan1(n, s_a, &cum);
-  const int most = s_long;
+  x.cum = block_excl_scan1(n, s_b, &cum);          // (its barrier also publishes s_long)
+  const bool whole = s_long <= kWhole;
   int at = tid;
-  if (most <= kWhole) {
-    // whole tiles: the longer half first, so that none of them begins last
-    int first;
+  if (whole) {
+    // by length; equal ones in any order
+    int rank = 0;
+    if (tid < rt) rank = atomicAdd(&s_count[n], 1);
     __syncthreads();
-    const int before = block_excl_scan1(2 * n > most, s_a, &first);
-    at = 2 * n > most ? before : first + tid - before;
+    for (int y = n + 1; y <= s_long; ++y) rank += s_count[y];
+    at = rank;
   }
   if (tid < rt) pl.tiles[at] = x;
   if (tid == 0) {
     pl.head[0] = cum;
     pl.head[1] = rt;
-    pl.head[2] = most <= kWhole ? 0 : min(fill, max(1, cum * a.hkv / kRun));
+    pl.head[2] = whole ? 0 : min(fill, max(1, cum * a.hkv / kRun));
   }
 }
 
 // Rows of the tiles whose units were dealt to several workgroups, kJoinRows of
-// them per workgroup.
-constexpr int kJoinRows = 16;
+// them at a time.
+constexpr int kJoinRows = 16, kJoinGrid = 8192;
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_join_tiles(DenseArgs a, Plan pl, Parts split) {
   constexpr int SL = kDenseRows / kJoinRows;
-  const int per = pl.head[0], ntiles = pl.head[1];
-  const int kvh = (int)blockIdx.x / (pl.limit * SL), x0 = (int)blockIdx.x % (pl.limit * SL);
-  const int it = x0 / SL, r0 = (x0 % SL) * kJoinRows;
-  if (it >= ntiles) return;
-  if (pl.head[2] == 0) return;
-  const Tile t = pl.tiles[it];
-  const int first = kvh * per + t.cum;
-  const int n = (it + 1 < ntiles ? pl.tiles[it + 1].cum : per) - t.cum;
-  const Deal deal(per * a.hkv, pl.head[2]);
-  const int w0 = deal.wg_of(first), w1 = deal.wg_of(first + n - 1);
-  if (w0 == w1) return;
-  int s0, s1;
-  rows_of(a, t.seq, s0, s1);
-  const int64_t row0 = (int64_t)t.tile * kDenseRows + r0;
-  const int nrow = (int)min((int64_t)kJoinRows, (int64_t)(s1 - s0) * a.g - row0);
+  const int per = pl.head[0], ntiles = pl.head[1], cut = pl.head[2];
+  if (cut == 0) return;
+  const Deal deal(per * a.hkv, cut);
+  for (int y = (int)blockIdx.x; y < ntiles * a.hkv * SL; y += (int)gridDim.x) {
+    const int r0 = (y % SL) * kJoinRows, it = y / SL % ntiles, kvh = y / SL / ntiles;
+    const Tile t = pl.tiles[it];
+    const int first = kvh * per + t.cum;
+    const int n = (it + 1 < ntiles ? pl.tiles[it + 1].cum : per) - t.cum;
+    const int w0 = deal.wg_of(first), w1 = deal.wg_of(first + n - 1);
+    if (w0 == w1) continue;
+    const int64_t row0 = (int64_t)t.tile * kDenseRows + r0;
+    const int nrow = (int)min((int64_t)kJoinRows, (int64_t)t.rows * a.g - row0);
 #pragma unroll 2
-  for (int x = threadIdx.x; x < nrow * (D / 4); x += 256) {
-    const int row = x / (D / 4), dc = x % (D / 4);
-    float m = -INFINITY, l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int x = threadIdx.x; x < nrow * (D / 4); x += 256) {
+      const int row = x / (D / 4), dc = x % (D / 4);
+      float m = -INFINITY, l = 0.f;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int w = w0; w <= w1; ++w) {
-      const int64_t pr = (2 * (int64_t)w + (w == w0 ? 1 : 0)) * kDenseRows + r0 + row;
-      const float mi = split.m[pr], li = split.l[pr], mx = fmaxf(m, mi);
-      const f32x4 oi = *reinterpret_cast<const f32x4*>(split.o + pr * D + 4 * dc);
-      const float f = part_weight(m, mx), fi = part_weight(mi, mx);
-      m = mx;
-      l = l * f + li * fi;
-      o = o * f + oi * fi;
+      for (int w = w0; w <= w1; ++w) {
+        const int64_t pr = (2 * (int64_t)w + (w == w0 ? 1 : 0)) * kDenseRows + r0 + row;
+        const float mi = split.m[pr], li = split.l[pr], mx = fmaxf(m, mi);
+        const f32x4 oi = *reinterpret_cast<const f32x4*>(split.o + pr * D + 4 * dc);
+        const float f = part_weight(m, mx), fi = part_weight(mi, mx);
+        m = mx;
+        l = l * f + li * fi;
+        o = o * f + oi * fi;
+      }
+      const int tok = t.s0 + (int)((row0 + row) / a.g);
+      const int head = kvh * a.g + (int)((row0 + row) % a.g);
+      store_out<T>(a.out + ((int64_t)tok * a.hq + head) * D + 4 * dc, o, l);
     }
-    const int tok = s0 + (int)((row0 + row) / a.g), head = kvh * a.g + (int)((row0 + row) % a.g);
-    store_out<T>(a.out + ((int64_t)tok * a.hq + head) * D + 4 * dc, o, l);
   }
 }
 
@@ -220,7 +224,7 @@ __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Par
   s_o[grp][dc] = o;
   __syncthreads();
   if (grp == 0) {
-#pragma unroll
+#pragma unroll 8
     for (int i = 1; i < NP; ++i) {
       const float mi = s_m[i], mx = fmaxf(m, mi);
       const float f = part_weight(m, mx), fi = part_weight(mi, mx);
@@ -260,9 +264,17 @@ static int64_t decode_units(const DenseShape& s) {
   const int g = s.hq / s.hkv, nc = (g + kDecodeRows - 1) / kDecodeRows;
   return (int64_t)s.requests * s.hkv * nc * (((int64_t)s.nb * s.b + kUnit - 1) / kUnit + 1);
 }
+// Two workgroups per CU keep the memory busy; at D = 256 one does, and only one
+// fits.  A few items alone are cut into fewer parts (32 each, but one workgroup
+// per CU at least), which the join is quicker with: one request of 16000 tokens, 8
+// KV heads, D = 128: 23.4 us with 512 workgroups, 21.1 with 256; 32 requests
+// of 200 to 2000 tokens: 26.3 and 28.2.
 static int decode_grid(const DenseShape& s) {
-  const int64_t u = decode_units(s);
-  return u < kFill ? (int)u : kFill;
+  const int nc = (s.hq / s.hkv + kDecodeRows - 1) / kDecodeRows;
+  const int64_t items = (int64_t)s.requests * s.hkv * nc, u = decode_units(s);
+  const int64_t want = s.d == 256 ? kFill / 2 : items * 32 < kFill / 2 ? kFill / 2 : items * 32;
+  const int64_t fill = want < kFill ? want : kFill;
+  return (int)(u < fill ? u : fill);
 }
 static int64_t tile_limit(const DenseShape& s) {
   const int ns = s.ngroups ? s.ngroups : s.requests;
@@ -287,11 +299,12 @@ constexpr int64_t kDirectTiles = 2 * kFill, kDirectUnits = 8;
 static bool prefill_direct(const DenseShape& s) {
   const int tk = s.d == 256 ? 32 : 64;
   return !s.ngroups && (tile_limit(s) * s.hkv >= kDirectTiles ||
-                        (int64_t)s.nb * s.b <= kDirectUnits * tk);
+                        (int64_t)s.nb * s.b <= kDirectUnits * tk);   // (lists stay under 1024)
 }
 static int prefill_fill(const DenseShape& s) {
-  const int64_t u = prefill_units(s);
-  return u < kFill ? (int)u : kFill;
+  // k_shared holds one workgroup per CU at D = 256
+  const int64_t u = prefill_units(s), fill = s.ngroups && s.d == 256 ? kFill / 2 : kFill;
+  return (int)(u < fill ? u : fill);
 }
 // k_plan decides whether the tiles are cut: there are workgroups for both.
 static int prefill_grid(const DenseShape& s) {
@@ -314,15 +327,17 @@ static Parts take_parts(Carve& c, int64_t slots, int rows, int d) {
 // With groups there is no list of tiles: only the units before each group are kept.
 static size_t plan_bytes(const DenseShape& s) {
   if (s.ngroups) return stk_align((s.ngroups + 1) * sizeof(int32_t));
-  return stk_align(3 * sizeof(int32_t)) + stk_align((s.requests + 1) * sizeof(int32_t)) +
-         stk_align((size_t)tile_limit(s) * sizeof(Tile));
+  return stk_align(3 * sizeof(int32_t)) + stk_align((size_t)tile_limit(s) * sizeof(Tile));
 }
 static Plan take_plan(Carve& c, const DenseShape& s) {
   Plan p{};
   p.limit = (int)tile_limit(s);
-  if (!s.ngroups) p.head = c.take<int32_t>(3);
-  p.base = c.take<int32_t>((s.ngroups ? s.ngroups : s.requests) + 1);
-  if (!s.ngroups) p.tiles = c.take<Tile>(p.limit);
+  if (s.ngroups) {
+    p.base = c.take<int32_t>(s.ngroups + 1);
+  } else {
+    p.head = c.take<int32_t>(3);
+    p.tiles = c.take<Tile>(p.limit);
+  }
   return p;
 }
 
@@ -350,7 +365,8 @@ static int launch_plan(const DenseArgs& a, const Plan& p, int d, int fill, hipSt
 template <typename T>
 static void launch_join_tiles(const DenseArgs& a, const Plan& p, const Parts& split, int d,
                               hipStream_t st) {
-  const unsigned g = (unsigned)(p.limit * a.hkv * (kDenseRows / kJoinRows));
+  const int all = p.limit * a.hkv * (kDenseRows / kJoinRows);
+  const unsigned g = (unsigned)(all < kJoinGrid ? all : kJoinGrid);
   if (d == 64) k_join_tiles<T, 64><<<g, 256, 0, st>>>(a, p, split);
   else if (d == 128) k_join_tiles<T, 128><<<g, 256, 0, st>>>(a, p, split);
   else k_join_tiles<T, 256><<<g, 256, 0, st>>>(a, p, split);

@@ -108,14 +108,17 @@ __device__ __forceinline__ void rows_of(const DenseArgs& a, int r, int& s0, int&
   s1 = min(max(a.starts[r + 1], s0), a.t);
 }
 
-// Keys that query row t at position p of a request of n tokens sees.
-__device__ __forceinline__ Span span_of(const DenseArgs& a, int r, int t, int p, int n) {
+// Keys that a query row of request r sees, at position p of n tokens and with
+// its document from `first` on.
+__device__ __forceinline__ Span span_at(const DenseArgs& a, int r, int first, int p, int n) {
   Span s;
-  s.lo = a.window > 0 ? max(0, p - a.window + 1) : 0;
-  if (a.first) s.lo = max(s.lo, a.first[t]);
+  s.lo = max(a.window > 0 ? max(0, p - a.window + 1) : 0, first);
   s.hi = min(p + 1, n);
   if (a.prefix) s.hi = max(s.hi, min(a.prefix[r], n));
   return s;
+}
+__device__ __forceinline__ Span span_of(const DenseArgs& a, int r, int t, int p, int n) {
+  return span_at(a, r, a.first ? a.first[t] : 0, p, n);
 }
 
 // Shared leading keys of request r (0 outside every group).
@@ -202,8 +205,8 @@ struct Deal {
 struct Tile { int seq, tile, kstart, cum, klo, khi, max_lo, min_hi, s0, rows, len; };
 struct Plan {
   int32_t* head;      // {units per KV head, tiles, workgroups that the units are dealt to (0: tiles are whole)}
-  int32_t* base;      // [sequences + 1] first tile of each sequence
   Tile* tiles;
+  int32_t* base;      // with groups, instead of a list: [groups + 1] units before each
   int limit;          // most tiles there can be
 };
 

@@ -49,21 +49,26 @@ __device__ __forceinline__ int decode_chunks(const DenseArgs& a) {
 // the first unit of workgroup `wg` of `launched`, and the units before that
 // request (past the last workgroup with work: any).  Workgroup 0 also leaves
 // the units before every request, and their total, in place [R + 1] for k_join_rows.
-struct DecodePlace { int total, base, r; };
+struct DecodePlace { int total, base, r; DecodeSpan span; };
 
 __device__ __forceinline__ DecodePlace decode_place(const DenseArgs& a, int wg, int launched,
                                                     int32_t* place) {
   __shared__ int s_tmp[4], s_at[2];
+  __shared__ DecodeSpan s_span;
   const int per = a.hkv * decode_chunks(a);
   int total = 0, c0 = 0, b0 = 0, sum0 = 0;
+  DecodeSpan span{}, span0{};
   for (int r0 = 0; r0 < a.requests; r0 += 256) {
     const int r = r0 + (int)threadIdx.x;
-    const int c = r < a.requests ? decode_span(a, r).n * per : 0;
+    span.n = 0;
+    if (r < a.requests) span = decode_span(a, r);
+    const int c = span.n * per;
     int sum;
     __syncthreads();
     const int before = total + block_excl_scan1(c, s_tmp, &sum);
     if (wg == 0 && r < a.requests) place[r] = before;
     if (r0 == 0) {
+      span0 = span;
       c0 = c;
       b0 = before;
       sum0 = sum;
@@ -76,19 +81,23 @@ __device__ __forceinline__ DecodePlace decode_place(const DenseArgs& a, int wg, 
   for (int r0 = 0; r0 < a.requests; r0 += 256) {
     const int r = r0 + (int)threadIdx.x;
     int c = c0, before = b0, sum = sum0;
+    span = span0;
     if (r0 > 0) {
-      c = r < a.requests ? decode_span(a, r).n * per : 0;
+      span.n = 0;
+      if (r < a.requests) span = decode_span(a, r);
+      c = span.n * per;
       __syncthreads();
       before = base + block_excl_scan1(c, s_tmp, &sum);
     }
     if (u >= before && u < before + c) {
       s_at[0] = before;
       s_at[1] = r;
+      s_span = span;
     }
     base += sum;
   }
   __syncthreads();
-  DecodePlace p{total, s_at[0], s_at[1]};
+  DecodePlace p{total, s_at[0], s_at[1], s_span};
   p.base = __builtin_amdgcn_readfirstlane(p.base);
   p.r = __builtin_amdgcn_readfirstlane(p.r);
   return p;
@@ -132,8 +141,9 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
     const int row = 4 * kg + (n16 >> 2);
     va[db] = row * D + (db ^ fsw(row)) * 16 + 4 * (n16 & 3);
   }
+  DecodeSpan next = at.span;
   while (u < u1) {
-    DecodeSpan sp = decode_span(a, r);
+    DecodeSpan sp = next;
     sp.lo = __builtin_amdgcn_readfirstlane(sp.lo);
     sp.hi = __builtin_amdgcn_readfirstlane(sp.hi);
     sp.lo16 = __builtin_amdgcn_readfirstlane(sp.lo16);
@@ -141,7 +151,7 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
     const int per = a.hkv * nc * sp.n;
     if (u >= base + per) {
       base += per;
-      ++r;
+      next = decode_span(a, ++r);
       continue;
     }
     const int item = (u - base) / sp.n, j0 = (u - base) % sp.n;

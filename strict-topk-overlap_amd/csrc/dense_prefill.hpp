@@ -116,6 +116,14 @@ __device__ void slow_rows(const DenseArgs& a, int seq, int s0, int s1, int64_t r
   }
 }
 
+// Workgroups of whole tiles come in the order of their length, and each CU takes
+// two: the first 256 one each, the next 256 the second ones.  Those are taken in
+// reverse, so that a CU's longest tile shares it with a short one.
+__device__ __forceinline__ int paired(int it, int n, int hkv) {
+  const int half = 256 / hkv, top = min(n, 2 * half);
+  return it >= half && it < top ? half + top - 1 - it : it;
+}
+
 // The tile of workgroup wg where every tile has its own.  Neighbouring
 // workgroups take one tile of each KV head, so that with eight heads (or a divisor of
 // eight) an XCD, to which every eighth workgroup goes, reads one head's keys;
@@ -125,7 +133,7 @@ struct TilePlace { int seq, tile, kvh; };
 
 __device__ __forceinline__ TilePlace tile_place(const DenseArgs& a, int wg, int nwg) {
   __shared__ int s_tmp[4], s_at[2];
-  const int it = wg / a.hkv;
+  const int it = paired(wg / a.hkv, nwg / a.hkv, a.hkv);
   int base = 0;
   if (threadIdx.x == 0) s_at[0] = -1;
   for (int r0 = 0; r0 < a.requests; r0 += 256) {
@@ -272,7 +280,7 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
     if (whole_tile) {                     // a tile each, dealt as tile_place does
       if (wg >= ntiles * a.hkv) return;
       kvh = wg % a.hkv;
-      it = wg / a.hkv;
+      it = paired(wg / a.hkv, ntiles, a.hkv);
     } else {
       const Deal deal(per * a.hkv, cut);
       if ((uint32_t)wg >= deal.grid) return;

@@ -491,7 +491,7 @@ size_t stk_paged_attention_workspace_bytes(int tokens, int requests, int hq, int
  * whatever they hold.  out [tokens, Hq, D] has the pages' type; its rows of
  * no request are left as they are, or zeroed with fill != 0.  ragged (of the
  * workspace query) says whether starts is given.  Shapes: FP16 / BF16, D in
- * {64, 128, 256}, B a multiple of 16, scale > 0. */
+ * {64, 128, 256}, B a multiple of 16, scale in (0, 1e30], softcap at most 4096. */
 int stk_paged_attention(const void* q, int64_t q_stride, int dtype, int tokens, int requests,
                         int hq, int hkv, int nb, int b, int d, int pages, const void* k_pages,
                         const void* v_pages, const int32_t* block_table, const int32_t* nblocks,

@@ -167,19 +167,25 @@ __device__ __forceinline__ void join_parts(const Parts& p, int i0, int count, in
   }
 }
 
-// One (request, query head) of a decode batch: the parts of its own keys, and
-// with SHARED those of its group's shared keys.
-template <typename T, int D, bool SHARED>
+// One row, (request, query head) of a decode batch, per workgroup or, where
+// there are enough of them (`WAVE`), per wave: the parts of its own keys, and with
+// SHARED those of its group's shared keys.  Bound by latency (a row's loads are four
+// dependent rounds, about 5 us): 3072 rows of 23 parts took two rounds of
+// workgroups, 13 us, and take 11 as waves; 2560 of 22 at D = 64 11 and 7.6.
+template <typename T, int D, bool SHARED, bool WAVE>
 __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Parts whole,
                                                    const int32_t* place, int launched, Plan pl,
                                                    Parts psplit, Parts pwhole, int plaunched) {
-  constexpr int CH = D / 4, NP = 256 / CH;       // 4-wide columns, parts in flight
+  constexpr int CH = D / 4, NP = (WAVE ? STK_WAVE : 256) / CH;   // 4-wide columns, parts in flight
   __shared__ float s_m[NP], s_l[NP];
   __shared__ f32x4 s_o[NP][CH];
-  const int r = (int)blockIdx.x / a.hq, head = (int)blockIdx.x % a.hq;
+  const int x = WAVE ? (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(wave_id())
+                     : (int)blockIdx.x;
+  if (WAVE && x >= a.requests * a.hq) return;
+  const int r = x / a.hq, head = x % a.hq;
   const int kvh = head / a.g, gi = head % a.g, nc = decode_chunks(a);
   const int item = kvh * nc + gi / kDecodeRows, hrow = gi % kDecodeRows;
-  const int dc = threadIdx.x % CH, grp = threadIdx.x / CH;
+  const int tid = WAVE ? lane_id() : (int)threadIdx.x, dc = tid % CH, grp = tid / CH;
   // a request has the same units for each of its items
   const int base = place[r], end = place[r + 1], total = place[a.requests];
   const int n = (end - base) / (a.hkv * nc), first = base + item * n;
@@ -217,23 +223,38 @@ __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Par
       }
     }
   }
-  if (dc == 0) {
-    s_m[grp] = m;
-    s_l[grp] = l;
-  }
-  s_o[grp][dc] = o;
-  __syncthreads();
-  if (grp == 0) {
-#pragma unroll 8
-    for (int i = 1; i < NP; ++i) {
-      const float mi = s_m[i], mx = fmaxf(m, mi);
+  if constexpr (WAVE) {
+#pragma unroll
+    for (int d = CH; d < STK_WAVE; d <<= 1) {
+      const float mi = __shfl_xor(m, d), li = __shfl_xor(l, d), mx = fmaxf(m, mi);
       const float f = part_weight(m, mx), fi = part_weight(mi, mx);
       m = mx;
-      l = l * f + s_l[i] * fi;
-      o = o * f + s_o[i][dc] * fi;
+      l = l * f + li * fi;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float oi = __shfl_xor(o[i], d);
+        o[i] = o[i] * f + oi * fi;
+      }
     }
-    store_out<T>(a.out + ((int64_t)r * a.hq + head) * D + 4 * dc, o, l);
+  } else {
+    if (dc == 0) {
+      s_m[grp] = m;
+      s_l[grp] = l;
+    }
+    s_o[grp][dc] = o;
+    __syncthreads();
+    if (grp == 0) {
+#pragma unroll
+      for (int i = 1; i < NP; ++i) {
+        const float mi = s_m[i], mx = fmaxf(m, mi);
+        const float f = part_weight(m, mx), fi = part_weight(mi, mx);
+        m = mx;
+        l = l * f + s_l[i] * fi;
+        o = o * f + s_o[i][dc] * fi;
+      }
+    }
   }
+  if (grp == 0) store_out<T>(a.out + ((int64_t)r * a.hq + head) * D + 4 * dc, o, l);
 }
 
 // ------------------------------------------------------------------ host
@@ -372,13 +393,17 @@ static void launch_join_tiles(const DenseArgs& a, const Plan& p, const Parts& sp
   else k_join_tiles<T, 256><<<g, 256, 0, st>>>(a, p, split);
 }
 
+constexpr unsigned kJoinAlone = 1024;   // rows that have a workgroup each
 template <typename T, bool SHARED>
 static void launch_join_rows(const DenseArgs& a, const Parts& split, const Parts& whole,
                              const int32_t* place, int grid, const Plan& p, const Parts& ps,
                              const Parts& pw, int pgrid, int d, hipStream_t st) {
-  const unsigned g = (unsigned)(a.requests * a.hq);
-#define STK_JOIN(D) \
-  k_join_rows<T, D, SHARED><<<g, 256, 0, st>>>(a, split, whole, place, grid, p, ps, pw, pgrid)
+  const unsigned rows = (unsigned)(a.requests * a.hq);
+#define STK_JOIN(D)                                                                               \
+  (rows <= kJoinAlone ? k_join_rows<T, D, SHARED, false><<<rows, 256, 0, st>>>(                   \
+                            a, split, whole, place, grid, p, ps, pw, pgrid)                       \
+                      : k_join_rows<T, D, SHARED, true><<<(rows + 3) / 4, 256, 0, st>>>(          \
+                            a, split, whole, place, grid, p, ps, pw, pgrid))
   if (d == 64) STK_JOIN(64);
   else if (d == 128) STK_JOIN(128);
   else STK_JOIN(256);
@@ -423,6 +448,11 @@ static int run_dense(const DenseShape& s, DenseArgs a, int mode, void* workspace
   return stk_check_launch("k_join_rows");
 }
 
+// A cap's tanh is 1 - 2 / (1 + e^2y), within 2^-23 of the true value whatever its
+// size: the capped score is within 2^-23 cap, which at 4096 is 2^-11, half a step
+// of FP16.  (A cap far above the scores caps nothing; with no cap there is no such term.)
+constexpr float kMaxScale = 1e30f, kMaxCap = 4096.f;
+
 static int dense(const DenseShape& s, const void* q, int64_t q_stride, int dtype, int pages,
                  const void* k_pages, const void* v_pages, const int32_t* table,
                  const int32_t* nblocks, const int32_t* ntokens, const int32_t* starts,
@@ -433,9 +463,9 @@ static int dense(const DenseShape& s, const void* q, int64_t q_stride, int dtype
   STK_REQUIRE(s.ragged || s.tokens == s.requests, "expected one query token per request");
   STK_REQUIRE(s.tokens == 0 || (q && out), "null pointer");
   STK_REQUIRE(k_pages && v_pages && table && nblocks, "null pointer");
-  STK_REQUIRE(scale > 0.f && scale <= 3.402823466e38f, "scale must be positive and finite");
-  STK_REQUIRE(softcap >= 0.f && softcap <= 3.402823466e38f,
-              "softcap must be finite, 0 for none");
+  STK_REQUIRE(scale > 0.f && scale <= kMaxScale, "scale must be positive and at most 1e30");
+  STK_REQUIRE(softcap >= 0.f && softcap <= kMaxCap && (softcap == 0.f || scale / softcap <= kMaxScale),
+              "softcap must be in (0, 4096], 0 for none, and not far below the scale");
   STK_REQUIRE(window >= 0, "window must be at least 0 (0: none)");
   STK_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) |
                 reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) &

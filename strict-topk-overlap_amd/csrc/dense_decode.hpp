@@ -259,19 +259,24 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
           for (int i = 0; i < DB; ++i) acc[i] *= f;
         }
         const float ms = m == -INFINITY ? 0.f : m;
-        u16x8 p;
+        // P in two 16-bit parts: the second product then keeps the weights nearly as the
+        // sum has them, and the matrix instructions have time to spare here
+        u16x8 p, pr;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float e = __builtin_amdgcn_exp2f(x[i] - ms);
           l += e;
           p[i] = to16<T>(e);
+          pr[i] = to16<T>(e - cvt(T{p[i]}));
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
           const u16x4 lo = lds_tr(vt + va[db]), hi = lds_tr(vt + va[db] + 16 * D);
-          acc[db] = mma16<T>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), p, acc[db]);
+          const u16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          acc[db] = mma16<T>(v, p, acc[db]);
+          acc[db] = mma16<T>(v, pr, acc[db]);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();

@@ -438,8 +438,8 @@ PyObject* attention_impl(PyObject* const* a, Py_ssize_t n) {
   double scale = 1.0 / std::sqrt((double)p.d), cap;
   int window;
   if ((a[9] != Py_None && !plain_float(a[9], &scale)) || !plain_float(a[10], &cap) ||
-      !plain_int(a[12], 0, 0x7fffffff, &window) || !(scale > 0) || !(cap >= 0) ||
-      std::isinf(scale) || std::isinf(cap))
+      !plain_int(a[12], 0, 0x7fffffff, &window) || !(scale > 0) || !(scale <= 1e30) ||
+      !(cap >= 0) || !(cap <= 4096))
     Py_RETURN_NONE;
   if ((st && !int_vector(*st, p.r + 1)) || (!st && t != p.r) || (pre && !int_vector(*pre, p.r)) ||
       (fir && !int_vector(*fir, t)) ||

@@ -313,10 +313,10 @@ def _dense_args(q, kv, scale, softcap, slopes, window, first, out):
         raise ValueError("Hq must be divisible by Hkv")
     scale = d ** -0.5 if scale is None else float(scale)
     softcap = float(softcap or 0.0)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError("scale must be positive and finite")
-    if not 0.0 <= softcap < float("inf"):
-        raise ValueError("softcap must be finite and at least 0 (0: none)")
+    if not 0.0 < scale <= 1e30:
+        raise ValueError("scale must be positive and at most 1e30")
+    if not 0.0 <= softcap <= 4096.0:
+        raise ValueError("softcap must be at least 0 (0: none) and at most 4096")
     window = int(window or 0)
     if not 0 <= window < 2 ** 31:
         raise ValueError("window must be at least 0 (0: none)")
@@ -364,7 +364,7 @@ def attention(q, kv, starts=None, scale=None, softcap=0.0, slopes=None, window=0
     that is causal attention, with ``window`` over the nearest keys, with
     ``prefix`` tokens that see each other both ways, with ``first`` the start of the
     token's document.  Scores are scale q.k (scale 1 / sqrt(D) by default),
-    capped to softcap * tanh(. / softcap) when ``softcap`` > 0, less
+    capped to softcap * tanh(. / softcap) when ``softcap`` > 0 (at most 4096), less
     slopes[h] * |p - j| with ``slopes`` (float32 [Hq]).  A token that sees no
     key gets zeros; what it does not see does not reach it, whatever the
     cache holds there.

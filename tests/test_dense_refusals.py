@@ -47,7 +47,8 @@ COMMON = [(dict(dtype=0), "FP16 or BF16"), (dict(d=96), "64, 128 or 256"),
           (dict(q=None), "null"), (dict(kp=None), "null"), (dict(nblocks=None), "null"),
           (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"),
           (dict(scale=float("inf")), "scale"), (dict(softcap=-1.0), "softcap"),
-          (dict(softcap=float("nan")), "softcap"), (dict(window=-1), "window"),
+          (dict(softcap=float("nan")), "softcap"), (dict(softcap=4097.0), "softcap"),
+          (dict(softcap=1e-35), "softcap"), (dict(scale=2e30), "scale"), (dict(window=-1), "window"),
           (dict(q=X + 2), "aligned"), (dict(qs=511), "aligned"), (dict(ws=None), "workspace"),
           (dict(bytes=16), "workspace"), (dict(pages=1 << 30), "too large"),
           (dict(nb=1 << 26), "too large"), (dict(pages=0), "bad shape")]

@@ -36,17 +36,21 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(DenseArgs a, Plan pl, int
   s_base[tid] = block_excl_scan1(mine, s_a, &base);
   __syncthreads();
   const int rt = min(min(base, pl.limit), kPlanThreads);
+  // four threads look at a tile's tokens where there are enough
+  const int lanes = a.first && 4 * rt <= kPlanThreads ? 4 : 1;
+  const int it = tid / lanes, sub = tid % lanes;
+  const bool lists = it < rt && sub == 0;
   Tile x{};
   int n = 0, cum;
-  if (tid < rt) {
+  if (it < rt) {
     int lo = 0, hi = ns - 1;             // last request that begins at or before this tile
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
-      if (s_base[mid] <= tid) lo = mid;
+      if (s_base[mid] <= it) lo = mid;
       else hi = mid - 1;
     }
     x.seq = lo;
-    x.tile = (lo + 1 < ns ? s_base[lo + 1] : base) - 1 - tid;
+    x.tile = (lo + 1 < ns ? s_base[lo + 1] : base) - 1 - it;
     x.s0 = s_s0[lo];
     x.rows = s_rows[lo];
     x.len = s_len[lo];
@@ -66,17 +70,32 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(DenseArgs a, Plan pl, int
       x.min_hi = some ? min(x.min_hi, s.hi) : 0;
     };
     if (a.first) {
-      for (int t = t0; t <= t1; t += 16) {
-        int f[16];
+      for (int t = t0 + sub; t <= t1; t += 8 * lanes) {
+        int f[8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = a.first[min(t + i, t1)];
+        for (int i = 0; i < 8; ++i) f[i] = a.first[min(t + i * lanes, t1)];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) see(min(t + i, t1), f[i]);
+        for (int i = 0; i < 8; ++i) {
+          // (past the end: the last token again)
+          const int y = min(t + i * lanes, t1);
+          see(y, f[i]);
+        }
       }
     } else {                             // the spans of a request's tokens only move up
       see(t0, 0);
       see(t1, 0);
     }
+  }
+  if (lanes > 1) {
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      x.klo = min(x.klo, __shfl_xor(x.klo, o));
+      x.khi = max(x.khi, __shfl_xor(x.khi, o));
+      x.max_lo = max(x.max_lo, __shfl_xor(x.max_lo, o));
+      x.min_hi = min(x.min_hi, __shfl_xor(x.min_hi, o));
+    }
+  }
+  if (lists) {
     if (x.khi <= x.klo) x.klo = x.khi = 0;
     x.kstart = x.klo & ~15;
     n = max(1, (x.khi - x.kstart + tk - 1) / tk);
@@ -84,16 +103,16 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(DenseArgs a, Plan pl, int
   }
   x.cum = block_excl_scan1(n, s_b, &cum);          // (its barrier also publishes s_long)
   const bool whole = s_long <= kWhole;
-  int at = tid;
+  int at = it;
   if (whole) {
     // by length; equal ones in any order
     int rank = 0;
-    if (tid < rt) rank = atomicAdd(&s_count[n], 1);
+    if (lists) rank = atomicAdd(&s_count[n], 1);
     __syncthreads();
     for (int y = n + 1; y <= s_long; ++y) rank += s_count[y];
     at = rank;
   }
-  if (tid < rt) pl.tiles[at] = x;
+  if (lists) pl.tiles[at] = x;
   if (tid == 0) {
     pl.head[0] = cum;
     pl.head[1] = rt;
@@ -472,7 +491,8 @@ static int dense(const DenseShape& s, const void* q, int64_t q_stride, int dtype
                15) == 0 && q_stride % 8 == 0 && q_stride >= 0,
               "rows must be 16-byte aligned");
   STK_REQUIRE(decode_units(s) <= 0x7fffffff && (int64_t)s.requests * s.hq <= 0x7fffffff &&
-                  most_units(s) <= 0x7fffffff,
+                  most_units(s) <= 0x7fffffff &&
+                  (int64_t)s.tokens * (s.hq / s.hkv) + kDenseRows <= 0x7fffffff,
               "batch too large");
   STK_REQUIRE(workspace && workspace_bytes >= dense_bytes(s), "workspace too small");
   STK_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0,

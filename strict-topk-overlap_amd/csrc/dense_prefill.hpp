@@ -257,6 +257,7 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
 
   int u = 0, u1 = 1, kvh, it = 0, per = 0, ntiles = 0, gbase = 0;
   TilePlace mine{0, 0, 0};
+  Tile alone{};
   bool whole_tile = KIND == DIRECT;
   if constexpr (KIND == DIRECT) {
     mine = tile_place(a, wg, nwg);
@@ -276,11 +277,13 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
     per = pl.head[0];
     ntiles = pl.head[1];
     const int cut = pl.head[2];
+    // a whole tile's entry is requested beside the head
+    kvh = wg % a.hkv;
+    it = min(paired(wg / a.hkv, pl.limit, a.hkv), pl.limit - 1);
+    alone = pl.tiles[it];
     whole_tile = cut == 0;
     if (whole_tile) {                     // a tile each, dealt as tile_place does
-      if (wg >= ntiles * a.hkv) return;
-      kvh = wg % a.hkv;
-      it = paired(wg / a.hkv, ntiles, a.hkv);
+      if (it >= ntiles || wg >= pl.limit * a.hkv) return;
     } else {
       const Deal deal(per * a.hkv, cut);
       if ((uint32_t)wg >= deal.grid) return;
@@ -321,7 +324,7 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
   while (u < u1) {
     Tile tl{mine.seq, mine.tile, 0, 0, 0, 0, 0, 0, 0, 0, 0};
     int units = 0;
-    if constexpr (KIND == LISTED) tl = pl.tiles[it];
+    if constexpr (KIND == LISTED) tl = whole_tile ? alone : pl.tiles[it];
     if constexpr (KIND == GROUPED) {
       if (u == (kvh + 1) * per) {                     // the next KV head's first group
         ++kvh;
@@ -350,10 +353,11 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
     }
     const int s0 = __builtin_amdgcn_readfirstlane(tl.s0);
     const int nrow = __builtin_amdgcn_readfirstlane(tl.rows);
-    const int64_t rown = (int64_t)tile * kDenseRows + 32 * w + n32;
-    const bool valid = rown < (int64_t)nrow * a.g;
-    const int tok = s0 + (int)(valid ? rown / a.g : 0);
-    const int head = kvh * a.g + (int)(valid ? rown % a.g : 0);
+    const uint32_t rown = (uint32_t)tile * kDenseRows + 32 * w + n32;   // (T G fits an int)
+    const bool valid = rown < (uint32_t)nrow * (uint32_t)a.g;
+    const uint32_t rtok = valid ? rown / (uint32_t)a.g : 0;
+    const int tok = s0 + (int)rtok;
+    const int head = kvh * a.g + (valid ? (int)(rown - rtok * (uint32_t)a.g) : 0);
     u16x8 qf[KS];
     const uint16_t* qp = a.q + (int64_t)tok * a.qs + (int64_t)head * D + 8 * h;
 #pragma unroll
@@ -538,17 +542,24 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
                   *reinterpret_cast<const u16x8*>(lk + (kb ^ (32 * x)) + 64 * b * D), qf[x], s[b]);
         }
       }
-      // MODE 0 keeps the products as they are: their scale goes into the exponent's FMA
-      const float sc = MODE ? 1.f : a.c;
-      if constexpr (MODE != 0) {
+      // Scores are kept as y, x = y sc + off in base 2, and sc and off go into the
+      // exponent's FMA: the products themselves, or -1 / (1 + e^2y) of a capped one
+      const float sc = MODE == 0 ? a.c : MODE == 1 ? 2.f * a.cap_out : 1.f;
+      const float off = MODE == 1 ? a.cap_out : 0.f;
+      if constexpr (MODE == 1) {
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            s[b][x] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(s[b][x] * a.cap_in));
+      } else if constexpr (MODE != 0) {
         const float dist = (float)(p - key0 - 4 * h);
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const int off = 32 * b + 8 * (x / 4) + x % 4;
-            s[b][x] = score2<MODE>(a, s[b][x], slope, dist - (float)off);
-          }
+          for (int x = 0; x < 16; ++x)
+            s[b][x] = score2<MODE>(a, s[b][x], slope,
+                                   dist - (float)(32 * b + 8 * (x / 4) + x % 4));
       }
       if (edge) {
         // key0 + 4 h + off in [lo, hi), as one unsigned comparison
@@ -572,7 +583,7 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
       for (int b = 0; b < KB; ++b)
 #pragma unroll
         for (int x = 0; x < 16; ++x) top = fmaxf(top, s[b][x]);
-      top *= sc;
+      top = __builtin_fmaf(top, sc, off);
       if (__any(top > m + kLazy)) {
         float mx = fmaxf(top, m);
         mx = fmaxf(mx, __shfl_xor(mx, 32));
@@ -582,12 +593,12 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
 #pragma unroll
         for (int i = 0; i < DB; ++i) acc[i] *= f;
       }
-      const float ms = m == -INFINITY ? 0.f : m;
+      const float ms = off - (m == -INFINITY ? 0.f : m);
 #pragma unroll
       for (int b = 0; b < KB; ++b)
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][x], sc, -ms));
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][x], sc, ms));
           l += e;
           pf[2 * b + x / 8][x % 8] = to16<T>(e);
         }

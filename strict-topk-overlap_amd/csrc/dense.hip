@@ -6,14 +6,26 @@ namespace stk {
 
 constexpr int kPlanThreads = 1024;     // and the most requests and tiles that are listed
 
-// A tile of up to kWhole units is not worth cutting.  Cut tiles leave parts that
-// k_join_tiles has to read (64 KB per cut at D = 128), and each workgroup begins
-// twice; whole ones leave part of the device idle while the longest one ends.
-// Causal prompts, 32 query heads over 8 KV heads, D = 128: 1024 tokens 54 us
-// cut, 37 whole; 2048 tokens (longest tile 32 units) 95 cut, 65 whole.
-constexpr int kWhole = 40;
-// Cut tiles are dealt in runs of at least kRun units.
-constexpr int kRun = 4;
+// Cut tiles are dealt in runs of at least kRun units; whole ones have at most
+// kWhole (for which there is room to sort them).
+constexpr int kRun = 4, kWhole = 1024;
+
+// Whether `units` units in tiles of at most `most` are better left whole.  A unit
+// takes about 1.4 us on a CU of its own and 2 beside another workgroup (`fill` of
+// them on 256 CUs).  Whole tiles last as long as the longest one, or as all of
+// them dealt out and half the longest one's tail; cut ones are even, but leave
+// parts that k_join_tiles has to read, and each workgroup begins twice: 20 us, and
+// 25 more where every workgroup does.  Causal prompts, 32 query heads over 8 KV
+// heads, D = 128: 1024 tokens (longest tile 16 units) 54 us cut, 37 whole; 2048
+// tokens 95 cut, 65 whole; 471 tokens of 4 heads at D = 256 (33 units, 16
+// tiles) 78 whole.
+__device__ __forceinline__ bool leave_whole(int units, int most, int fill) {
+  const int wgs = min(fill, max(1, units / kRun));
+  const float unit = wgs <= 256 ? 1.4f : 2.f;
+  const float whole = fmaxf(1.4f * most, 2.f * units / fill + 0.7f * most);
+  const float cut = unit * units / wgs + 20.f + 25.f * wgs / 512.f;
+  return whole <= cut && most <= kWhole;
+}
 
 // Lists the row tiles: one workgroup.  Within a request the last rows, which see
 // the most keys, come first; whole tiles are listed by their length, the longest
@@ -21,10 +33,11 @@ constexpr int kRun = 4;
 __global__ __launch_bounds__(kPlanThreads) void k_plan(DenseArgs a, Plan pl, int tk, int fill) {
   __shared__ int s_a[kPlanThreads / STK_WAVE], s_b[kPlanThreads / STK_WAVE], s_long;
   __shared__ int s_base[kPlanThreads + 1], s_s0[kPlanThreads], s_rows[kPlanThreads],
-      s_len[kPlanThreads], s_count[kWhole + 1];
+      s_len[kPlanThreads], s_count[kWhole + 2];
   const int tid = threadIdx.x, ns = a.requests;
   if (tid == 0) s_long = 0;
-  if (tid <= kWhole) s_count[tid] = 0;
+  s_count[tid] = 0;
+  if (tid < 2) s_count[kPlanThreads + tid] = 0;
   int s0 = 0, s1 = 0, base;
   if (tid < ns) {
     rows_of(a, tid, s0, s1);
@@ -102,15 +115,19 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(DenseArgs a, Plan pl, int
     atomicMax(&s_long, n);
   }
   x.cum = block_excl_scan1(n, s_b, &cum);          // (its barrier also publishes s_long)
-  const bool whole = s_long <= kWhole;
+  const bool whole = leave_whole(cum * a.hkv, s_long, fill);
   int at = it;
   if (whole) {
-    // by length; equal ones in any order
-    int rank = 0;
+    // by length, the longest first; equal ones in any order
+    int rank = 0, all;
     if (lists) rank = atomicAdd(&s_count[n], 1);
     __syncthreads();
-    for (int y = n + 1; y <= s_long; ++y) rank += s_count[y];
-    at = rank;
+    // tiles longer than kWhole - tid, by a prefix sum over the lengths from the top
+    const int here = s_count[kWhole - tid];
+    const int longer = block_excl_scan1(here, s_a, &all);
+    s_base[tid] = longer;
+    __syncthreads();
+    if (lists) at = s_base[kWhole - n] + rank;
   }
   if (lists) pl.tiles[at] = x;
   if (tid == 0) {
@@ -230,7 +247,7 @@ __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Par
       const int tile = (int)(idx / kDenseRows), rr = (int)(idx % kDenseRows);
       const int units = group_units(a, g, kTk<D>), per = pl.base[a.ngroups];
       const int pf = kvh * per + pl.base[g] + tile * units;
-      const Deal pdeal(per * a.hkv, plaunched);
+      const Deal pdeal(per * a.hkv, group_grid(per * a.hkv, kTk<D>, plaunched));
       const int v0 = pdeal.wg_of(pf), v1 = pdeal.wg_of(pf + units - 1);
       if (v0 == v1) {
         const int64_t at = group_slot(a, kvh, g, s0, tile, pl.limit) * kDenseRows + rr;
@@ -304,15 +321,14 @@ static int64_t decode_units(const DenseShape& s) {
   const int g = s.hq / s.hkv, nc = (g + kDecodeRows - 1) / kDecodeRows;
   return (int64_t)s.requests * s.hkv * nc * (((int64_t)s.nb * s.b + kUnit - 1) / kUnit + 1);
 }
-// Two workgroups per CU keep the memory busy; at D = 256 one does, and only one
-// fits.  A few items alone are cut into fewer parts (32 each, but one workgroup
-// per CU at least), which the join is quicker with: one request of 16000 tokens, 8
-// KV heads, D = 128: 23.4 us with 512 workgroups, 21.1 with 256; 32 requests
-// of 200 to 2000 tokens: 26.3 and 28.2.
+// A few items alone are cut into fewer parts (32 each, but one workgroup per CU at
+// least), which the join is quicker with: one request of 16000 tokens, 8 KV
+// heads, D = 128: 23.4 us with 512 workgroups, 21.1 with 256; 32 requests of 200
+// to 2000 tokens: 26.3 and 28.2.
 static int decode_grid(const DenseShape& s) {
   const int nc = (s.hq / s.hkv + kDecodeRows - 1) / kDecodeRows;
   const int64_t items = (int64_t)s.requests * s.hkv * nc, u = decode_units(s);
-  const int64_t want = s.d == 256 ? kFill / 2 : items * 32 < kFill / 2 ? kFill / 2 : items * 32;
+  const int64_t want = items * 32 < kFill / 2 ? kFill / 2 : items * 32;
   const int64_t fill = want < kFill ? want : kFill;
   return (int)(u < fill ? u : fill);
 }
@@ -342,9 +358,8 @@ static bool prefill_direct(const DenseShape& s) {
                         (int64_t)s.nb * s.b <= kDirectUnits * tk);   // (lists stay under 1024)
 }
 static int prefill_fill(const DenseShape& s) {
-  // k_shared holds one workgroup per CU at D = 256
-  const int64_t u = prefill_units(s), fill = s.ngroups && s.d == 256 ? kFill / 2 : kFill;
-  return (int)(u < fill ? u : fill);
+  const int64_t u = prefill_units(s);
+  return u < kFill ? (int)u : kFill;
 }
 // k_plan decides whether the tiles are cut: there are workgroups for both.
 static int prefill_grid(const DenseShape& s) {
@@ -412,7 +427,7 @@ static void launch_join_tiles(const DenseArgs& a, const Plan& p, const Parts& sp
   else k_join_tiles<T, 256><<<g, 256, 0, st>>>(a, p, split);
 }
 
-constexpr unsigned kJoinAlone = 1024;   // rows that have a workgroup each
+constexpr unsigned kJoinAlone = 2048;   // rows that have a workgroup each: one round of them
 template <typename T, bool SHARED>
 static void launch_join_rows(const DenseArgs& a, const Parts& split, const Parts& whole,
                              const int32_t* place, int grid, const Plan& p, const Parts& ps,

@@ -9,7 +9,7 @@
 // the host.
 //
 // Within a workgroup the four waves take a quarter of the keys each and share
-// nothing until the item ends.  A wave's tile is 32 keys:
+// nothing until the item ends.  A wave's tile is 32 keys (at D = 256 it is 16):
 //   S[key, head] = K Q^T  (16x16x32, K straight from global memory to registers,
 //                          in the operand's own layout),
 //   O^T[dim, head] += V^T P^T  (V through the wave's own LDS, read transposed).
@@ -103,19 +103,24 @@ __device__ __forceinline__ DecodePlace decode_place(const DenseArgs& a, int wg, 
   return p;
 }
 
-template <int D> constexpr size_t kDecodeLds = 4 * sizeof(uint16_t) * 32 * D;
+// At D = 256 a tile of 32 keys and the next one's rows would leave a wave per SIMD.
+template <int D> constexpr int kDecodeTile = D == 256 ? 16 : 32;
+// a wave's V tile, and after its last one its output rows in FP32
+template <int D> constexpr size_t kDecodeWave = 64 * D;
+template <int D> constexpr size_t kDecodeLds = 4 * kDecodeWave<D>;
 
 // The work of workgroup wg of nwg.  With PARTS items that lie whole in it leave
 // their parts in `whole`, too, instead of being finished.
 template <typename T, int D, int MODE, bool PARTS>
 __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, const Parts& whole,
                                        int32_t* place, char* lds, int wg, int nwg) {
+  constexpr int TW = kDecodeTile<D>;    // keys per tile
+  constexpr int HW = TW / 16;           // its runs of 16 keys
   constexpr int KS = D / 32;            // QK steps
   constexpr int DB = D / 16;            // output blocks
-  constexpr int VN = D / 16;            // 16-byte chunks of a V tile per lane
+  constexpr int VN = TW * D / 512;      // 16-byte chunks of a V tile per lane
   constexpr int CPR = D / 8;            // chunks per row
   constexpr int RPI = STK_WAVE / CPR;   // rows per load instruction
-  uint16_t* const s_v = reinterpret_cast<uint16_t*>(lds);         // [4][32 * D]
   __shared__ float s_m[4][16], s_l[4][16];
   const int lane = lane_id(), w = wave_id();
   const int n16 = lane & 15, kg = lane >> 4;
@@ -129,7 +134,7 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
   // V tile in LDS: row-major, 32-byte blocks swizzled so that the 16 rows of a
   // transposed read spread over all banks
   auto fsw = [](int row) { return D == 64 ? (row >> 1) & 3 : row & 7; };
-  uint16_t* vt = s_v + w * (32 * D);
+  uint16_t* vt = reinterpret_cast<uint16_t*>(lds + w * kDecodeWave<D>);
   int vw[VN], va[DB];
 #pragma unroll
   for (int i = 0; i < VN; ++i) {
@@ -174,80 +179,83 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
 #pragma unroll
     for (int i = 0; i < DB; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    const int nt = kb > ka ? (kb - ka + 31) / 32 : 0, tpw = (nt + 3) / 4;
+    const int nt = kb > ka ? (kb - ka + TW - 1) / TW : 0, tpw = (nt + 3) / 4;
     const int ta = w * tpw, tb = min(nt, ta + tpw);
     if (ta < tb) {
-      const int wk = ka + 32 * ta;                      // the wave's first key
+      const int wk = ka + TW * ta;                      // the wave's first key
       auto window = [&](int i) {                        // rows of 64 runs of 16 keys
         const int key = wk + 16 * (64 * i + lane);
         const int x = pool_row(a, row, min(key, kb));
         return key < kb ? x : -1;
       };
       int ent = window(0), nxt = window(1);
-      u16x8 kf[2][KS], vf[VN];
-      int r0, r1;
+      u16x8 kf[HW][KS], vf[VN];
+      int rw[HW];
       auto load = [&](int t) {
-        if (t > 0 && (t & 31) == 0) {
+        if (t > 0 && (HW * t) % 64 == 0) {
           ent = nxt;
-          nxt = window(t / 32 + 1);
+          nxt = window(HW * t / 64 + 1);
         }
-        r0 = __builtin_amdgcn_readlane(ent, (2 * t) & 63);
-        r1 = __builtin_amdgcn_readlane(ent, (2 * t + 1) & 63);
-        const int64_t p0 = (int64_t)max(r0, 0) * D, p1 = (int64_t)max(r1, 0) * D;
-        const int ko = n16 * D + 8 * kg;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          kf[0][s] = *reinterpret_cast<const u16x8*>(a.kp + p0 + ko + 32 * s);
-          kf[1][s] = *reinterpret_cast<const u16x8*>(a.kp + p1 + ko + 32 * s);
+        for (int y = 0; y < HW; ++y) rw[y] = __builtin_amdgcn_readlane(ent, (HW * t + y) & 63);
+#pragma unroll
+        for (int y = 0; y < HW; ++y) {
+          const uint16_t* kr = a.kp + (int64_t)max(rw[y], 0) * D + n16 * D + 8 * kg;
+#pragma unroll
+          for (int s = 0; s < KS; ++s) kf[y][s] = *reinterpret_cast<const u16x8*>(kr + 32 * s);
         }
 #pragma unroll
         for (int i = 0; i < VN; ++i) {
           const int vr = i * RPI;                       // rows vr .. vr + RPI - 1
           vf[i] = *reinterpret_cast<const u16x8*>(
-              a.vp + (vr < 16 ? p0 : p1) + ((vr & 15) + lane / CPR) * D + 8 * (lane % CPR));
+              a.vp + (int64_t)max(rw[vr / 16], 0) * D + ((vr & 15) + lane / CPR) * D +
+              8 * (lane % CPR));
         }
       };
       load(0);
       const int cnt = tb - ta;
       for (int t = 0; t < cnt; ++t) {
-        const int key0 = wk + 32 * t;
-        const bool full = key0 >= sp.lo && key0 + 32 <= kb && r0 >= 0 && r1 >= 0;
+        const int key0 = wk + TW * t;
+        bool full = key0 >= sp.lo && key0 + TW <= kb;
+#pragma unroll
+        for (int y = 0; y < HW; ++y) full = full && rw[y] >= 0;
         if (!full) {
           // keys that are not seen: their values are not read as numbers
 #pragma unroll
           for (int i = 0; i < VN; ++i) {
             const int kr = i * RPI + lane / CPR, key = key0 + kr;
-            const bool ok = key >= sp.lo && key < kb && (kr < 16 ? r0 : r1) >= 0;
+            const bool ok = key >= sp.lo && key < kb && rw[i * RPI / 16] >= 0;
             if (!ok) vf[i] = u16x8{};
           }
         }
-        const int rr0 = r0, rr1 = r1;
+        int was[HW];
+#pragma unroll
+        for (int y = 0; y < HW; ++y) was[y] = rw[y];
 #pragma unroll
         for (int i = 0; i < VN; ++i) *reinterpret_cast<u16x8*>(vt + vw[i]) = vf[i];
-        f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+        f32x4 sq[HW];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          s0 = mma16<T>(kf[0][s], qf[s], s0);
-          s1 = mma16<T>(kf[1][s], qf[s], s1);
-        }
+        for (int y = 0; y < HW; ++y) sq[y] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int y = 0; y < HW; ++y) sq[y] = mma16<T>(kf[y][s], qf[s], sq[y]);
         if (t + 1 < cnt) load(t + 1);
-        float x[8];
+        float x[4 * HW];
         const float dist = (float)(sp.hi - 1 - key0 - 4 * kg);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = score2<MODE>(a, s0[i], slope, dist - (float)i);
-          x[4 + i] = score2<MODE>(a, s1[i], slope, dist - (float)(16 + i));
-        }
+        for (int i = 0; i < 4 * HW; ++i)
+          x[i] = score2<MODE>(a, sq[i / 4][i % 4], slope, dist - (float)(16 * (i / 4) + i % 4));
         if (!full) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = key0 + 4 * kg + i;
-            x[i] = key >= sp.lo && key < kb && rr0 >= 0 ? x[i] : -INFINITY;
-            x[4 + i] = key + 16 >= sp.lo && key + 16 < kb && rr1 >= 0 ? x[4 + i] : -INFINITY;
+          for (int i = 0; i < 4 * HW; ++i) {
+            const int key = key0 + 4 * kg + 16 * (i / 4) + i % 4;
+            x[i] = key >= sp.lo && key < kb && was[i / 4] >= 0 ? x[i] : -INFINITY;
           }
         }
-        const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                                fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        float top = x[0];
+#pragma unroll
+        for (int i = 1; i < 4 * HW; ++i) top = fmaxf(top, x[i]);
         if (__any(top > m + kLazy)) {
           float mx = fmaxf(top, m);
           mx = fmaxf(mx, __shfl_xor(mx, 16));
@@ -261,9 +269,9 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
         const float ms = m == -INFINITY ? 0.f : m;
         // P in two 16-bit parts: the second product then keeps the weights nearly as the
         // sum has them, and the matrix instructions have time to spare here
-        u16x8 p, pr;
+        uint16_t p[8], pr[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4 * HW; ++i) {
           const float e = __builtin_amdgcn_exp2f(x[i] - ms);
           l += e;
           p[i] = to16<T>(e);
@@ -271,12 +279,24 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+        if constexpr (HW == 2) {
+          const u16x8 ph = {p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]};
+          const u16x8 pl = {pr[0], pr[1], pr[2], pr[3], pr[4], pr[5], pr[6], pr[7]};
 #pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          const u16x4 lo = lds_tr(vt + va[db]), hi = lds_tr(vt + va[db] + 16 * D);
-          const u16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-          acc[db] = mma16<T>(v, p, acc[db]);
-          acc[db] = mma16<T>(v, pr, acc[db]);
+          for (int db = 0; db < DB; ++db) {
+            const u16x4 lo = lds_tr(vt + va[db]), hi = lds_tr(vt + va[db] + 16 * D);
+            const u16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            acc[db] = mma16<T>(v, ph, acc[db]);
+            acc[db] = mma16<T>(v, pl, acc[db]);
+          }
+        } else {
+          // sixteen keys fill one product: both parts of P against the same V
+          const u16x8 pp = {p[0], p[1], p[2], p[3], pr[0], pr[1], pr[2], pr[3]};
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            const u16x4 v = lds_tr(vt + va[db]);
+            acc[db] = mma16<T>(__builtin_shufflevector(v, v, 0, 1, 2, 3, 4, 5, 6, 7), pp, acc[db]);
+          }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -312,7 +332,7 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
         const float f = part_weight(mi, mx);
         sum += f * s_l[i][h];
         o += f * *reinterpret_cast<const f32x4*>(
-                     reinterpret_cast<const float*>(s_v + i * (32 * D)) + h * D + 4 * dc);
+                     reinterpret_cast<const float*>(lds + i * kDecodeWave<D>) + h * D + 4 * dc);
       }
       if (keep) {
         store_out<T>(a.out + ((int64_t)r * a.hq + h0 + h) * D + 4 * dc, o, sum);
@@ -330,7 +350,7 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
 }
 
 template <typename T, int D, int MODE>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_decode(DenseArgs a, Parts split,
+__global__ __launch_bounds__(256, 2) void k_decode(DenseArgs a, Parts split,
                                                                   int32_t* place) {
   __shared__ __attribute__((aligned(16))) char lds[kDecodeLds<D>];
   decode<T, D, MODE, false>(a, split, split, place, lds, (int)blockIdx.x, (int)gridDim.x);

@@ -172,6 +172,15 @@ __device__ __forceinline__ int group_units(const DenseArgs& a, int g, int tk) {
 }
 struct GroupPlace { int per, g, base; };      // per = 0: no work
 
+// Workgroups that the groups' units are dealt to, of those launched, in runs of at
+// least two units: each run leaves a part of up to 128 rows to write and read.
+// At D = 256, where units are smaller and parts larger, four, and beyond one
+// workgroup per CU sixteen.
+__device__ __forceinline__ int group_grid(int units, int tk, int launched) {
+  const int most = tk == 64 ? units / 2 : max(min(units / 4, 256), units / 16);
+  return min(launched, max(1, most));
+}
+
 __device__ __forceinline__ GroupPlace group_place(const DenseArgs& a, int& wg, int launched, int tk,
                                                   int32_t* place) {
   __shared__ int s_tmp[4], s_at[2];
@@ -188,7 +197,7 @@ __device__ __forceinline__ GroupPlace group_place(const DenseArgs& a, int& wg, i
     per += sum;
   }
   if (wg == 0 && threadIdx.x == 0) place[a.ngroups] = per;
-  const Deal deal(per * a.hkv, launched);
+  const Deal deal(per * a.hkv, group_grid(per * a.hkv, tk, launched));
   if ((uint32_t)wg >= deal.grid) return GroupPlace{0, 0, 0};
   wg = xcd_remap(wg, (int)deal.grid);
   const int u = deal.at(wg) % per;
@@ -269,7 +278,7 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
     per = at.per;
     it = at.g;
     gbase = at.base;
-    const Deal deal(per * a.hkv, nwg);
+    const Deal deal(per * a.hkv, group_grid(per * a.hkv, TK, nwg));
     u = deal.at(wg);
     u1 = deal.at(wg + 1);
     kvh = u / per;

@@ -12,7 +12,7 @@
 namespace stk {
 
 template <typename T, int D, int MODE>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_shared(DenseArgs a, Plan pl, Parts psplit,
+__global__ __launch_bounds__(256, 2) void k_shared(DenseArgs a, Plan pl, Parts psplit,
                                                                   Parts pwhole, int pgrid,
                                                                   Parts split, Parts whole,
                                                                   int32_t* place) {

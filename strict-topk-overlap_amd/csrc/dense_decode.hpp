@@ -18,7 +18,9 @@
 // 16 + 4g .. 16 + 4g + 3} as its eight, P never leaves its lane.
 // The next tile's K and V are in flight while a tile is worked on.
 //
-// Bound by HBM: every key and value is read once (per 16 query heads of its KV head).
+// Bound by HBM: every key and value is read once (per 16 query heads of its KV
+// head).  16 requests of 8192 to 131000 tokens, 8 KV heads, D = 128: 2.6 GB in 434 us, 6.0
+// TB/s; one request of 16000 tokens 15 us, of which 5 pass before its first tile.
 #pragma once
 
 #include "dense.hpp"

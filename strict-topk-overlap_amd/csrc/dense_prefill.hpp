@@ -15,6 +15,14 @@
 // LDS rows are swizzled (16-byte chunks of K, 64-byte blocks of V) so that
 // neither read has bank conflicts.
 //
+// Bound by the SIMDs: of an 8192-token causal prompt (32 query heads over 8, D =
+// 128: 530 us, 1.03 PFLOP/s, where the card's library product reaches 1.19) the
+// matrix instructions take 51 % and the softmax's 47 %; at D = 256 1040 us, 1.06.
+// P is rounded to 16 bits for the second product, the sum of its weights is not:
+// relative error 0.0020 of the prompt's output, 0.0015 of which is the output's own
+// rounding.  A second part of P, as k_decode has, would be half as many matrix
+// instructions again.
+//
 // Masks are one range of keys per row; units that every row of the tile sees whole
 // (all but the first and last ones) skip them.  In the others the values that no
 // row sees are zeroed in LDS; should a value that some rows see and others do

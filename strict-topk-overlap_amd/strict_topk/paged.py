@@ -27,6 +27,13 @@ results are those of the dense steps on the request's own blocks, bit for
 bit, except that a request with fewer blocks than ``topk`` selects all of them
 (the rest of its ID row is -1).  A table entry outside [0, P) is an invalid page: its block
 scores lowest and has the empty state, and nothing is read from it.
+
+Around those steps a serving loop runs the dense operators over the same pool:
+``extend`` writes any number of new tokens per request, rotated to their
+positions, ``attention`` lets them see their whole cache (prompts, chunks of
+prompts, single tokens; capped or distance-biased scores; window, prefix and document
+masks), and ``shared_attention`` is its form for requests that share leading
+blocks.
 """
 from __future__ import annotations
 

@@ -420,3 +420,109 @@ def test_refusals():
     with pytest.raises(ValueError):
         paged.attention(odd, kv)
     assert paged.attention(q[:0], kv, torch.zeros(3, **ints)).shape == (0, 4, 64)
+
+
+# ------------------------------------------- tiles that are listed, and cut
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("mask", ["none", "window", "prefix", "first", "all"])
+def test_listed_tiles(d, mask):
+    """Short requests in a wide table: the tiles are listed on the device and taken whole."""
+    lens, news = [300, 0, 90, 150, 33, 600], [170, 0, 90, 1, 33, 64]
+    kv = R.make(2, d, 32, lens, BF, width=400)
+    q = R.queries(sum(news), 10, d, BF)
+    pos = [n - m + t for n, m in zip(lens, news) for t in range(m)]
+    ints = dict(dtype=torch.int32, device="cuda")
+    kw = {}
+    if mask in ("window", "all"):
+        kw["window"] = 70
+    if mask in ("prefix", "all"):
+        kw["prefix"] = torch.tensor([200, 5, 1000, -5, 33, 580], **ints)
+    if mask in ("first", "all"):
+        first = [p // 37 * 37 for p in pos]
+        first[3], first[5], first[100], first[171] = -7, pos[5] + 1, 2 ** 31 - 1, 500
+        kw["first"] = torch.tensor(first, **ints)
+    _run(q, kv, news, **kw)
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("dtype,hq,hkv,d,b", [(BF, 8, 2, 128, 32), (FP, 3, 1, 64, 16),
+                                              (BF, 6, 1, 256, 64)])
+def test_cut_tiles(dtype, hq, hkv, d, b, mode):
+    """Few long tiles: their keys are cut over many workgroups and the parts joined."""
+    lens, news = [2600, 700, 1500, 31], [20, 3, 61, 1]
+    kv = R.make(hkv, d, b, lens, dtype, width=200)
+    q = R.queries(sum(news), hq, d, dtype)
+    _run(q, kv, news, **_kw(hq, mode))
+
+
+@pytest.mark.parametrize("mask", ["window", "prefix", "first", "pages"])
+def test_cut_tiles_masks(mask):
+    lens, news = [2600, 1500], [30, 61]
+    kv = R.make(1, 128, 16, lens, FP, width=300)
+    q = R.queries(sum(news), 5, 128, FP)
+    ints = dict(dtype=torch.int32, device="cuda")
+    kw = {}
+    if mask == "window":
+        kw["window"] = 1333
+    if mask == "prefix":
+        kw["prefix"] = torch.tensor([2590, 1470], **ints)
+    if mask == "first":
+        kw["first"] = torch.tensor([(37 * i) % 2700 for i in range(sum(news))], **ints)
+    if mask == "pages":
+        kv.block_table[0, 0, 20:130:7] = -1
+        kv.block_table[1, 0, ::2] = kv.pages
+    _run(q, kv, news, **kw)
+
+
+def test_cut_tiles_hidden_places():
+    """A value that is no number, seen by some rows of a cut tile, reaches those rows alone."""
+    lens, news = [2600], [100]
+    kv = R.make(1, 64, 16, lens, BF, width=300)
+    q = R.queries(100, 2, 64, BF)
+    starts = R.starts_of(news)
+    ref, tol = R.attention(q, kv, news)
+    page = int(kv.block_table[0, 0, 2560 // 16])
+    kv.v_pages[page, 2560 % 16, 9] = float("nan")      # row t stands at 2500 + t
+    got = paged.attention(q, kv, starts)
+    R.check(got[:60], ref[:60], tol[:60])
+    keep = [i for i in range(64) if i != 9]
+    R.check(got[60:][..., keep], ref[60:][..., keep], tol[60:][..., keep])
+    assert bool(got[60:, :, 9].isnan().all())
+
+
+def test_output_over_the_queries():
+    """out may be q itself."""
+    lens, news = [2600, 90], [20, 90]
+    kv = R.make(2, 128, 16, lens, BF, width=200)
+    q = R.queries(110, 8, 128, BF)
+    starts = R.starts_of(news)
+    want = paged.attention(q, kv, starts)
+    assert torch.equal(paged.attention(q, kv, starts, out=q), want)
+    one = R.queries(2, 8, 128, BF)
+    want = paged.attention(one, kv)
+    assert torch.equal(paged.attention(one, kv, out=one), want)
+
+
+def test_malformed_starts_and_groups_stay_in_bounds():
+    """starts and groups that decrease or leave the rows give some result, and an intact cache."""
+    kv = R.make(2, 64, 16, [700, 90, 40], BF, width=60)
+    q = R.queries(40, 4, 64, BF)
+    keep = [x.clone() for x in (kv.k_pages, kv.v_pages, kv.block_table)]
+    ints = dict(dtype=torch.int32, device="cuda")
+    for s in ([0, 30, 10, 40], [5, 1000, -7, 40], [40, 40, 40, 40], [-5, -5, 50, 60],
+              [0, 40, 0, 40]):
+        paged.attention(q, kv, torch.tensor(s, **ints))
+        paged.extend(_scratch(kv), q[:, :2], q[:, 2:], torch.tensor(s, **ints),
+                     torch.tensor([3, 4, 5], **ints))
+    for g, n in (([0, 3, 1], [2, 2]), ([2, -4, 9], [1000, 3]), ([0, 3, 0, 3], [5, -1, 40])):
+        paged.shared_attention(q[:3], kv, torch.tensor(g, **ints), torch.tensor(n, **ints))
+    torch.cuda.synchronize()
+    for x, y in zip(keep, (kv.k_pages, kv.v_pages, kv.block_table)):
+        assert torch.equal(x, y)
+    R.check(paged.attention(q[:3], kv), *R.attention(q[:3], kv, [1] * 3))
+
+
+def _scratch(kv):
+    return paged.PagedKV(*(x.clone() for x in (kv.k_pages, kv.v_pages, kv.lo_pages, kv.hi_pages,
+                                               kv.block_table, kv.nblocks, kv.ntokens)))

@@ -348,14 +348,24 @@ static int64_t most_units(const DenseShape& s) {
   const int64_t rows = (int64_t)s.requests * (s.hq / s.hkv);
   return (prefill_units(s) / tile_limit(s)) * (rows / kDenseRows + 1) * s.ngroups;
 }
-// Tiles that fill the device several times over need no splitting, and neither do
-// those of caches that hold few units: without it there is nothing to list and
-// nothing to join.
-constexpr int64_t kDirectTiles = 2 * kFill, kDirectUnits = 8;
+// Without cutting there is nothing to list and nothing to join, which saves 7 to 12 us.
+// A cache that holds few units leaves little to cut.  Requests of several tiles
+// each fill the device evenly: so do they if there is a tile for every CU and the cache holds
+// a few more units, or tiles enough to fill it several times over.  More than
+// k_plan's tiles are not listed.
+// Measured (listed, direct): prompts of 1024 tokens, 32 query heads over 8 KV heads,
+// 36.5, 30 us, of 2048 64, 55.5; 32 requests of 16 tokens after up to 620 29, 22.  With
+// larger caches a tile per CU is not enough: 2900 tokens of 3 requests after up to
+// 12000 418, 574.  128 requests of 4 tokens, one of them after 60000 tokens and the others 500:
+// 153, 1171, and 375, 358 after 4000 each, so short requests are listed.
+constexpr int64_t kDirectUnits = 32, kEvenUnits = 64, kEvenTiles = 4;
 static bool prefill_direct(const DenseShape& s) {
   const int tk = s.d == 256 ? 32 : 64;
-  return !s.ngroups && (tile_limit(s) * s.hkv >= kDirectTiles ||
-                        (int64_t)s.nb * s.b <= kDirectUnits * tk);   // (lists stay under 1024)
+  const int64_t tiles = tile_limit(s), holds = (int64_t)s.nb * s.b;
+  if (s.ngroups) return false;
+  if (tiles > kPlanThreads || holds <= kDirectUnits * tk) return true;
+  return tiles >= kEvenTiles * s.requests &&
+         tiles * s.hkv >= (holds <= kEvenUnits * tk ? kFill / 2 : 2 * kFill);
 }
 static int prefill_fill(const DenseShape& s) {
   const int64_t u = prefill_units(s);

@@ -45,7 +45,8 @@ __device__ __forceinline__ bool nonfinite16(u16x8 v, uint16_t expo) {
 // (wave-uniform) on.  Counted by vmcnt like any load; the compiler does not
 // know of the write, so the caller waits (copies_done) and passes a barrier
 // before it reads.  (Its own intrinsic makes the compiler wait for all of these
-// before every LDS read.)
+// before every LDS read.  m0 is set beside each copy, and nothing else in these
+// kernels uses it.)
 __device__ __forceinline__ void copy_to_lds(uint32_t lds, const uint16_t* base, uint32_t off) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :

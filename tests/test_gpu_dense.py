@@ -456,6 +456,24 @@ def test_cut_tiles(dtype, hq, hkv, d, b, mode):
     _run(q, kv, news, **_kw(hq, mode))
 
 
+@pytest.mark.parametrize("long", [0, 5000])
+def test_many_short_tiles(long):
+    """More tiles than workgroups fill the device, of requests with one tile each, listed
+    whole and, beside one long request, cut."""
+    lens, news = [40 + 3 * (i % 50) for i in range(140)], [1 + i % 4 for i in range(140)]
+    lens[70] += long
+    kv = R.make(8, 64, 32, lens, BF, width=170)
+    _run(R.queries(sum(news), 16, 64, BF), kv, news)
+
+
+@pytest.mark.parametrize("requests", [1016, 1017])
+def test_most_listed_requests(requests):
+    """The most tiles that are listed, and more."""
+    lens, news = [1 + i % 90 for i in range(requests)], [1] * requests
+    kv = R.make(1, 64, 32, lens, FP, width=80)
+    _run(R.queries(requests, 1, 64, FP), kv, news, ragged=True)
+
+
 @pytest.mark.parametrize("mask", ["window", "prefix", "first", "pages"])
 def test_cut_tiles_masks(mask):
     lens, news = [2600, 1500], [30, 61]

@@ -421,6 +421,28 @@ __device__ __forceinline__ int block_excl_scan1(int v, int* tmp, int* total) {
   return before + inc - v;
 }
 
+// The last i in [0, n) with base(i) <= w, or -1; base does not decrease (if it does,
+// some i or -1).  The whole wave takes part, w is the same in all lanes: a round narrows
+// the range 256 times, so up to 256 entries cost one trip to memory, 65536 two.
+template <typename F>
+__device__ __forceinline__ int last_at_most(int n, int w, F base) {
+  int lo = 0;
+  for (;;) {
+    const int step = (n + 4 * STK_WAVE - 1) / (4 * STK_WAVE);
+    int at[4], c = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      at[j] = base(lo + min((j * STK_WAVE + lane_id()) * step, n - 1));
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      c += __popcll(__ballot((j * STK_WAVE + lane_id()) * step < n && at[j] <= w));
+    if (c == 0) return -1;
+    lo += (c - 1) * step;
+    if (step == 1) return lo;
+    n = min(step, n - (c - 1) * step);
+  }
+}
+
 __device__ __forceinline__ uint64_t wave_or64(uint64_t v) {
   for (int off = 1; off < STK_WAVE; off <<= 1) v |= __shfl_xor(v, off);
   return v;

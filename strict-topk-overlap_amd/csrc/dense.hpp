@@ -125,11 +125,21 @@ __device__ __forceinline__ Span span_of(const DenseArgs& a, int r, int t, int p,
 __device__ __forceinline__ int shared_of(const DenseArgs& a, int g) {
   return (int)min((int64_t)min(max(a.shared[g], 0), a.nb) * a.b, (int64_t)0x7ffffff0);
 }
+// The group that holds request r, or -1: the last one that begins at or before it, found
+// in rounds that narrow the range eight times.
 __device__ __forceinline__ int group_of(const DenseArgs& a, int r) {
-  int g = -1;
-  for (int i = 0; i < a.ngroups; ++i)
-    if (r >= a.groups[i] && r < a.groups[i + 1]) g = i;
-  return g;
+  int lo = 0, n = a.ngroups;
+  while (n > 1) {
+    const int step = (n + 7) / 8;
+    int at[7], c = 0;
+#pragma unroll
+    for (int j = 0; j < 7; ++j) at[j] = a.groups[lo + min((j + 1) * step, n - 1)];
+#pragma unroll
+    for (int j = 0; j < 7; ++j) c += (j + 1) * step < n && at[j] <= r;
+    lo += c * step;
+    n = min(step, n - c * step);
+  }
+  return r >= a.groups[lo] && r < a.groups[lo + 1] ? lo : -1;
 }
 
 // Pool row (page * B + offset) of the 16 keys that start at key, or -1: an

@@ -58,45 +58,54 @@ __device__ __forceinline__ DecodePlace decode_place(const DenseArgs& a, int wg, 
   __shared__ int s_tmp[4], s_at[2];
   __shared__ DecodeSpan s_span;
   const int per = a.hkv * decode_chunks(a);
-  int total = 0, c0 = 0, b0 = 0, sum0 = 0;
-  DecodeSpan span{}, span0{};
-  for (int r0 = 0; r0 < a.requests; r0 += 256) {
-    const int r = r0 + (int)threadIdx.x;
-    span.n = 0;
-    if (r < a.requests) span = decode_span(a, r);
-    const int c = span.n * per;
-    int sum;
+  // requests per thread and pass: their loads are in flight together
+  const int e = a.requests > 256 ? 4 : 1, pass = 256 * e;
+  DecodeSpan span[4];
+  // units of this pass's requests before this thread's, and of all of them
+  auto scan = [&](int r0, int& before, int& sum) {
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = r0 + e * (int)threadIdx.x + j;
+      span[j].n = 0;
+      if (j < e && r < a.requests) span[j] = decode_span(a, r);
+      c += span[j].n * per;
+    }
     __syncthreads();
-    const int before = total + block_excl_scan1(c, s_tmp, &sum);
-    if (wg == 0 && r < a.requests) place[r] = before;
-    if (r0 == 0) {
-      span0 = span;
-      c0 = c;
-      b0 = before;
-      sum0 = sum;
+    before = block_excl_scan1(c, s_tmp, &sum);
+  };
+  int total = 0, before = 0, sum = 0;
+  for (int r0 = 0; r0 < a.requests; r0 += pass) {
+    scan(r0, before, sum);
+    if (wg == 0) {
+      int at = total + before;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = r0 + e * (int)threadIdx.x + j;
+        if (j < e && r < a.requests) place[r] = at;
+        at += span[j].n * per;
+      }
     }
     total += sum;
   }
   if (wg == 0 && threadIdx.x == 0) place[a.requests] = total;
   const int u = Deal(total, launched).at(wg);
   int base = 0;
-  for (int r0 = 0; r0 < a.requests; r0 += 256) {
-    const int r = r0 + (int)threadIdx.x;
-    int c = c0, before = b0, sum = sum0;
-    span = span0;
-    if (r0 > 0) {
-      span.n = 0;
-      if (r < a.requests) span = decode_span(a, r);
-      c = span.n * per;
-      __syncthreads();
-      before = base + block_excl_scan1(c, s_tmp, &sum);
-    }
-    if (u >= before && u < before + c) {
-      s_at[0] = before;
-      s_at[1] = r;
-      s_span = span;
+  for (int r0 = 0; r0 < a.requests; r0 += pass) {
+    if (a.requests > pass) scan(r0, before, sum);
+    int at = base + before;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = span[j].n * per;
+      if (u >= at && u < at + c) {
+        s_at[0] = at;
+        s_at[1] = r0 + e * (int)threadIdx.x + j;
+        s_span = span[j];
+      }
+      at += c;
     }
     base += sum;
+    if (u < base) break;
   }
   __syncthreads();
   DecodePlace p{total, s_at[0], s_at[1], s_span};

@@ -136,33 +136,49 @@ __device__ __forceinline__ int paired(int it, int n, int hkv) {
 // The tile of workgroup wg where every tile has its own.  Neighbouring
 // workgroups take one tile of each KV head, so that with eight heads (or a divisor of
 // eight) an XCD, to which every eighth workgroup goes, reads one head's keys;
-// and within a sequence the last rows, which see the most keys, come first.
+// and within a sequence the last rows, which see the most keys, come first.  Up to 256
+// requests' tiles are laid end to end (four requests of 1024 tokens, one after 16000: 360
+// us, 441 with gaps, which moved long tiles to one CU).  Those of more, which every
+// workgroup would have to add up, come after floor(s G / 128) + r others, s their
+// first row: request r has at least as many places as tiles then (4096 requests of one or
+// two tokens 808 us, 530).
 // kvh = Hkv: none.
 struct TilePlace { int seq, tile, kvh; };
 
 __device__ __forceinline__ TilePlace tile_place(const DenseArgs& a, int wg, int nwg) {
   __shared__ int s_tmp[4], s_at[2];
   const int it = paired(wg / a.hkv, nwg / a.hkv, a.hkv);
-  int base = 0;
-  if (threadIdx.x == 0) s_at[0] = -1;
-  for (int r0 = 0; r0 < a.requests; r0 += 256) {
-    const int r = r0 + (int)threadIdx.x;
+  auto tiles = [&](int rows) { return (int)(((int64_t)rows * a.g + kDenseRows - 1) / kDenseRows); };
+  int r = -1, tile = -1;
+  if (a.requests <= 256) {
     int s0 = 0, s1 = 0, sum;
-    if (r < a.requests) rows_of(a, r, s0, s1);
-    const int c = (int)(((int64_t)(s1 - s0) * a.g + kDenseRows - 1) / kDenseRows);
-    __syncthreads();
-    const int before = base + block_excl_scan1(c, s_tmp, &sum);
+    if ((int)threadIdx.x < a.requests) rows_of(a, threadIdx.x, s0, s1);
+    const int c = tiles(s1 - s0);
+    if (threadIdx.x == 0) s_at[0] = -1;
+    const int before = block_excl_scan1(c, s_tmp, &sum);
     if (it >= before && it < before + c) {
-      s_at[0] = r;
+      s_at[0] = threadIdx.x;
       s_at[1] = before + c - 1 - it;
     }
-    base += sum;
-    if (it < base) break;
+    __syncthreads();
+    r = s_at[0];
+    tile = s_at[1];
+  } else {
+    auto before = [&](int i) {
+      return (int)((int64_t)min(max(a.starts[i], 0), a.t) * a.g / kDenseRows) + i;
+    };
+    r = last_at_most(a.requests, it, before);
+    if (r >= 0) {
+      int s0, s1;
+      rows_of(a, r, s0, s1);
+      const int c = tiles(s1 - s0);
+      tile = before(r) + c - 1 - it;
+      if (tile < 0 || tile >= c) r = -1;
+    }
   }
-  __syncthreads();
-  const int r = __builtin_amdgcn_readfirstlane(s_at[0]);
+  r = __builtin_amdgcn_readfirstlane(r);
   if (r < 0) return TilePlace{0, 0, a.hkv};
-  return TilePlace{r, __builtin_amdgcn_readfirstlane(s_at[1]), wg % a.hkv};
+  return TilePlace{r, __builtin_amdgcn_readfirstlane(tile), wg % a.hkv};
 }
 
 // Shared blocks: every tile of a group has the same units, those of its
@@ -193,16 +209,32 @@ __device__ __forceinline__ int group_grid(int units, int tk, int launched) {
 __device__ __forceinline__ GroupPlace group_place(const DenseArgs& a, int& wg, int launched, int tk,
                                                   int32_t* place) {
   __shared__ int s_tmp[4], s_at[2];
-  auto units = [&](int g) {
-    return g < a.ngroups ? group_tiles(a, g) * group_units(a, g, tk) : 0;
-  };
-  int per = 0;
-  for (int g0 = 0; g0 < a.ngroups; g0 += 256) {
-    const int g = g0 + (int)threadIdx.x;
-    int sum;
+  // groups per thread and pass: their loads are in flight together
+  const int e = a.ngroups > 256 ? 4 : 1, pass = 256 * e;
+  int units[4];
+  auto scan = [&](int g0, int& before, int& sum) {
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int g = g0 + e * (int)threadIdx.x + j;
+      units[j] = j < e && g < a.ngroups ? group_tiles(a, g) * group_units(a, g, tk) : 0;
+      c += units[j];
+    }
     __syncthreads();
-    const int before = per + block_excl_scan1(units(g), s_tmp, &sum);
-    if (wg == 0 && g < a.ngroups) place[g] = before;
+    before = block_excl_scan1(c, s_tmp, &sum);
+  };
+  int per = 0, before = 0, sum = 0;
+  for (int g0 = 0; g0 < a.ngroups; g0 += pass) {
+    scan(g0, before, sum);
+    if (wg == 0) {
+      int at = per + before;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int g = g0 + e * (int)threadIdx.x + j;
+        if (j < e && g < a.ngroups) place[g] = at;
+        at += units[j];
+      }
+    }
     per += sum;
   }
   if (wg == 0 && threadIdx.x == 0) place[a.ngroups] = per;
@@ -211,16 +243,19 @@ __device__ __forceinline__ GroupPlace group_place(const DenseArgs& a, int& wg, i
   wg = xcd_remap(wg, (int)deal.grid);
   const int u = deal.at(wg) % per;
   int base = 0;
-  for (int g0 = 0; g0 < a.ngroups; g0 += 256) {
-    const int g = g0 + (int)threadIdx.x, c = units(g);
-    int sum;
-    __syncthreads();
-    const int before = base + block_excl_scan1(c, s_tmp, &sum);
-    if (u >= before && u < before + c) {
-      s_at[0] = g;
-      s_at[1] = before;
+  for (int g0 = 0; g0 < a.ngroups; g0 += pass) {
+    if (a.ngroups > pass) scan(g0, before, sum);
+    int at = base + before;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (u >= at && u < at + units[j]) {
+        s_at[0] = g0 + e * (int)threadIdx.x + j;
+        s_at[1] = at;
+      }
+      at += units[j];
     }
     base += sum;
+    if (u < base) break;
   }
   __syncthreads();
   return GroupPlace{per, __builtin_amdgcn_readfirstlane(s_at[0]),

@@ -9,15 +9,16 @@
 // rounded once to the pages' type, since that is what the cache holds.  Pairs
 // are (i, i + rot / 2), or (2i, 2i + 1) interleaved.
 //
-// One workgroup owns one (request, KV head, touched block): it writes the
+// One workgroup owns one (request, KV head, touched block), or of requests with
+// few tokens several heads of one: it writes the
 // block's new K and V rows and folds the rotated keys, as stored, into the
 // page's lo/hi, so the bounds need no atomics and do not depend on an order.
 // A block whose first new token has offset 0 starts its bounds over.  The
 // other workgroups rotate the queries, one wave per run of 16-byte chunks of one
 // token.  The host knows neither the lengths nor the positions (they stay on
 // the device, so a captured graph follows them): the grid covers the most
-// blocks that T tokens of R requests can touch, each workgroup finds its block by
-// a prefix sum over the requests, and those past the last one leave.
+// blocks that T tokens of R requests can touch, in places that follow from the starts
+// alone, each workgroup finds its request by a search, and those with no block leave.
 //
 // Bound by HBM: every new row is read once and written once.  8191 tokens of
 // 32 + 16 heads, D = 128, FP16: 204 MB in 35 us, 5.8 TB/s with the inputs in the
@@ -42,7 +43,7 @@ struct ExtendArgs {
   void* lo; void* hi; int lb;
   const int32_t* table;
   int32_t* nblocks; int32_t* ntokens;
-  int page_wgs;
+  int page_wgs, each;             // workgroups of blocks; each: one for every token
 };
 
 template <typename T> __device__ __forceinline__ uint16_t round16(float v);
@@ -120,75 +121,115 @@ __device__ __forceinline__ void request_rows(const ExtendArgs& a, int r, int& s0
   s1 = min(max(a.starts[r + 1], s0), a.t);
 }
 
+// Places of blocks before request r's: the host does not know which
+// blocks it touches, so there is one for every token, or where that is fewer n / B + 2 of
+// its n tokens, rounded so that they add up to T / B + 2 R.
+__device__ __forceinline__ int slot_of(const ExtendArgs& a, int r) {
+  const int s0 = min(max(a.starts[r], 0), a.t);
+  return a.each ? s0 : s0 / a.b + 2 * r;
+}
+
+// The block of place `want`: n new tokens of request r from row src on, at offset
+// off; n = 0: none.  The workgroup that `counts` for the request's first block
+// sets its counts where every touched block has a page for every KV head and every
+// new token fits.
+struct TouchedBlock { int r, blk, off, first, n; int64_t src; };
+
+__device__ __forceinline__ TouchedBlock touched_block(const ExtendArgs& a, int want, bool counts) {
+  const int64_t room = (int64_t)a.nb * a.b;
+  TouchedBlock x{};
+  x.r = last_at_most(a.requests, want, [&](int i) { return slot_of(a, i); });
+  if (x.r < 0) return x;
+  int s0, s1;
+  request_rows(a, x.r, s0, s1);
+  const int p0 = a.positions[x.r], k = want - slot_of(a, x.r);
+  const int64_t end = (int64_t)p0 + (s1 - s0), from = max(p0, 0), to = min(end, room);
+  if (from >= to || k < 0) return x;
+  x.blk = (int)from / a.b + k;
+  if (x.blk > (int)(to - 1) / a.b) return x;
+  x.first = max(p0, x.blk * a.b);                                   // first new position here
+  x.off = x.first - x.blk * a.b;
+  x.n = (int)(min(end, ((int64_t)x.blk + 1) * a.b) - x.first);
+  x.src = (int64_t)s0 + (x.first - p0);
+  if (counts && k == 0) {
+    bool ok = p0 >= 0 && end <= room;
+    if (ok) {
+      const int32_t* row = a.table + (int64_t)x.r * a.hkv * a.nb;
+      const int cnt = (int)(end - 1) / a.b - x.blk + 1;
+      for (int64_t i = threadIdx.x; i < (int64_t)cnt * a.hkv; i += 256) {
+        const int pg = row[(i / cnt) * a.nb + x.blk + i % cnt];
+        ok = ok && pg >= 0 && pg < a.pages;
+      }
+    }
+    if (__syncthreads_and(ok) && threadIdx.x == 0) {
+      a.nblocks[x.r] = (int)((end + a.b - 1) / a.b);
+      if (a.ntokens) a.ntokens[x.r] = (int)end;
+    }
+  }
+  return x;
+}
+
+// A block with a place of its own: few tokens.  16 bytes of a row per thread
+// and a KV head per D / 8 threads, token after token.
+template <typename T, int D, bool INTER>
+__device__ __forceinline__ void extend_few(const ExtendArgs& a) {
+  constexpr int CPR = D / 8, HP = 256 / CPR;
+  const int hgs = (a.hkv + HP - 1) / HP, hg = blockIdx.x % hgs;
+  const TouchedBlock x = touched_block(a, blockIdx.x / hgs, hg == 0);
+  const int c = threadIdx.x % CPR, kvh = hg * HP + (int)threadIdx.x / CPR;
+  if (x.n == 0 || kvh >= a.hkv) return;
+  const int page = a.table[((int64_t)x.r * a.hkv + kvh) * a.nb + x.blk];
+  if (page < 0 || page >= a.pages) return;
+  constexpr bool BF = __is_same(T, bf16s);
+  const size_t dst = ((size_t)page * a.b + x.off) * D + 8 * c, bo = (size_t)page * D + 8 * c;
+  const uint16_t* kin = a.k + x.src * a.ks + kvh * D;
+  const uint16_t* vin = a.v + x.src * a.vs + kvh * D + 8 * c;
+  const int half = a.rot / 2;
+  float lo[8], hi[8];
+  if (x.off) {
+    load_bound8(a.lo, bo, a.lb, BF, lo);
+    load_bound8(a.hi, bo, a.lb, BF, hi);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      lo[i] = INFINITY;
+      hi[i] = -INFINITY;
+    }
+  }
+  for (int t = 0; t < x.n; ++t) {
+    const u16x8 v = *reinterpret_cast<const u16x8*>(vin + t * a.vs);
+    const int64_t ang = (int64_t)(x.first + t) * half;
+    const u16x8 k = rotate8<T, INTER>(kin + t * a.ks, c, a.cos + ang, a.sin + ang, a.rot);
+    *reinterpret_cast<u16x8*>(a.vp + dst + (size_t)t * D) = v;
+    *reinterpret_cast<u16x8*>(a.kp + dst + (size_t)t * D) = k;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = cvt(T{k[i]});
+      lo[i] = __builtin_elementwise_minimum(lo[i], f);
+      hi[i] = __builtin_elementwise_maximum(hi[i], f);
+    }
+  }
+  store_bound8(a.lo, bo, a.lb, BF, lo);
+  store_bound8(a.hi, bo, a.lb, BF, hi);
+}
+
+// One KV head of a block: its rows side by side.
 template <typename T, int D, bool INTER>
 __device__ __forceinline__ void extend_block(const ExtendArgs& a) {
   constexpr int CPR = D / 8;            // 16-byte chunks per row
   constexpr int RP = 256 / CPR;         // rows per pass
   constexpr bool BF = __is_same(T, bf16s);
-  __shared__ int s_tmp[4], s_hit[5];
   __shared__ float s_lo[4][D], s_hi[4][D];
-  const int tid = threadIdx.x, kvh = blockIdx.x % a.hkv, want = blockIdx.x / a.hkv;
-  const int64_t room = (int64_t)a.nb * a.b;
-  // this workgroup's request and block
-  int base = 0;
-  if (tid == 0) s_hit[0] = -1;
-  for (int r0 = 0; r0 < a.requests; r0 += 256) {
-    const int r = r0 + tid;
-    int cnt = 0, s0 = 0, s1 = 0, b0 = 0, p0 = 0;
-    if (r < a.requests) {
-      request_rows(a, r, s0, s1);
-      p0 = a.positions[r];
-      const int64_t lo = max(p0, 0), hi = min((int64_t)p0 + (s1 - s0), room);
-      if (lo < hi) {
-        b0 = (int)lo / a.b;
-        cnt = (int)(hi - 1) / a.b - b0 + 1;
-      }
-    }
-    int total;
-    __syncthreads();
-    const int before = base + block_excl_scan1(cnt, s_tmp, &total);
-    if (want >= before && want < before + cnt) {
-      s_hit[0] = r;
-      s_hit[1] = s0;
-      s_hit[2] = s1;
-      s_hit[3] = b0 + (want - before);
-      s_hit[4] = p0;
-    }
-    base += total;
-    __syncthreads();
-    if (want < base) break;
-  }
-  const int r = s_hit[0];
-  if (r < 0) return;
-  const int s0 = s_hit[1], s1 = s_hit[2], blk = s_hit[3], p0 = s_hit[4];
-  const int first = max(p0, blk * a.b);                             // first new position here
-  const int off = first - blk * a.b;
-  const int n = (int)(min((int64_t)p0 + (s1 - s0), ((int64_t)blk + 1) * a.b) - first);
-  const int32_t* row = a.table + ((int64_t)r * a.hkv + kvh) * a.nb;
-  // the counts follow when every touched block has a page for every KV head
-  // and every new token fits
-  if (kvh == 0 && blk == max(p0, 0) / a.b) {
-    const int64_t end = (int64_t)p0 + (s1 - s0);
-    bool ok = p0 >= 0 && end <= room;
-    if (ok) {
-      const int cnt = (int)(end - 1) / a.b - blk + 1;
-      for (int64_t x = tid; x < (int64_t)cnt * a.hkv; x += 256) {
-        const int pg = row[(x / cnt) * a.nb + blk + x % cnt];
-        ok = ok && pg >= 0 && pg < a.pages;
-      }
-    }
-    if (__syncthreads_and(ok) && tid == 0) {
-      a.nblocks[r] = (int)((end + a.b - 1) / a.b);
-      if (a.ntokens) a.ntokens[r] = (int)end;
-    }
-  }
-  const int page = row[blk];
+  const int tid = threadIdx.x, kvh = blockIdx.x % a.hkv;
+  const TouchedBlock at = touched_block(a, blockIdx.x / a.hkv, kvh == 0);
+  const int n = at.n, off = at.off, first = at.first;
+  if (n == 0) return;
+  const int page = a.table[((int64_t)at.r * a.hkv + kvh) * a.nb + at.blk];
   if (page < 0 || page >= a.pages) return;
   const int c = tid % CPR, g = tid / CPR;
-  const int64_t src = (int64_t)s0 + (first - p0);                   // row of the first token here
   const size_t dst = ((size_t)page * a.b + off) * D + 8 * c;
-  const uint16_t* kin = a.k + src * a.ks + kvh * D;
-  const uint16_t* vin = a.v + src * a.vs + kvh * D + 8 * c;
+  const uint16_t* kin = a.k + at.src * a.ks + kvh * D;
+  const uint16_t* vin = a.v + at.src * a.vs + kvh * D + 8 * c;
   const int half = a.rot / 2;
   float lo[8], hi[8], olo[8], ohi[8];
 #pragma unroll
@@ -266,17 +307,12 @@ __device__ __forceinline__ void extend_queries(const ExtendArgs& a, int wg) {
   const int64_t x = (int64_t)wg * 4 + wave_id();
   if (x >= (int64_t)a.t * runs) return;
   const int t = (int)(x / runs), c0 = (int)(x % runs) * kQChunks;
-  // the requests that end at or before row t come before its own
-  int r = 0;
-  for (int r0 = 0; r0 < a.requests; r0 += STK_WAVE) {
-    const int i = r0 + lane_id();
-    const int e = a.starts[min(i, a.requests - 1) + 1];
-    r += __popcll(__ballot(i < a.requests && e <= t));
-  }
+  const int r = last_at_most(a.requests, t, [&](int i) { return a.starts[i]; });
   int64_t p = -1;
-  if (r < a.requests) {
-    const int s0 = a.starts[r];
-    if (s0 <= t) p = (int64_t)a.positions[r] + (t - s0);
+  if (r >= 0) {
+    int s0, s1;
+    request_rows(a, r, s0, s1);
+    if (t >= s0 && t < s1) p = (int64_t)a.positions[r] + (t - s0);
   }
   const bool ok = p >= 0 && p < a.rows;
   const uint16_t* q = a.q + t * a.qs;
@@ -295,8 +331,9 @@ __device__ __forceinline__ void extend_queries(const ExtendArgs& a, int wg) {
 
 template <typename T, int D, bool INTER>
 __global__ __launch_bounds__(256) void k_extend(ExtendArgs a) {
-  if ((int)blockIdx.x < a.page_wgs) extend_block<T, D, INTER>(a);
-  else extend_queries<T, D, INTER>(a, (int)blockIdx.x - a.page_wgs);
+  if ((int)blockIdx.x >= a.page_wgs) extend_queries<T, D, INTER>(a, (int)blockIdx.x - a.page_wgs);
+  else if (a.each) extend_few<T, D, INTER>(a);
+  else extend_block<T, D, INTER>(a);
 }
 
 template <typename T, int D>
@@ -357,12 +394,13 @@ STK_API int stk_paged_extend(const void* k_new, int64_t k_stride, const void* v_
   STK_REQUIRE(k_stride >= 0 && v_stride >= 0 && q_stride >= 0, "negative stride");
   STK_REQUIRE(!ntokens || ntokens != positions, "positions must not be the cache's ntokens");
   if (tokens == 0) return STK_OK;
-  // blocks that T tokens of R requests can touch: a request of n >= 1 tokens
-  // touches at most n, and at most (n - 1) / B + 2
-  const int64_t some = requests < tokens ? requests : tokens;
-  const int64_t touched = tokens / b + 2 * some < tokens ? tokens / b + 2 * some : tokens;
+  // a request of n >= 1 tokens touches at most n blocks, and at most (n - 1) / B + 2
+  const int64_t few = tokens / b + 2 * (int64_t)requests;
+  const bool each = tokens <= few;
+  const int heads = 256 / (d / 8);                // KV heads per workgroup of few tokens
+  const int64_t touched = each ? (int64_t)tokens * ((hkv + heads - 1) / heads) : few * hkv;
   const int64_t runs = q ? ((int64_t)hq * (d / 8) + kQChunks - 1) / kQChunks : 0;
-  const int64_t grid = touched * hkv + (tokens * runs + 3) / 4;
+  const int64_t grid = touched + (tokens * runs + 3) / 4;
   STK_REQUIRE(grid <= 0x7fffffff, "batch too large");
   ExtendArgs a{};
   a.k = static_cast<const uint16_t*>(k_new); a.v = static_cast<const uint16_t*>(v_new);
@@ -376,7 +414,7 @@ STK_API int stk_paged_extend(const void* k_new, int64_t k_stride, const void* v_
   a.kp = static_cast<uint16_t*>(k_pages); a.vp = static_cast<uint16_t*>(v_pages);
   a.lo = lo_pages; a.hi = hi_pages; a.lb = bounds_dtype != 0;
   a.table = block_table; a.nblocks = nblocks; a.ntokens = ntokens;
-  a.page_wgs = (int)(touched * hkv);
+  a.page_wgs = (int)touched; a.each = each;
   hipStream_t st = (hipStream_t)stream;
   if (dtype == DT_BF16) launch_extend<bf16s>(a, d, interleaved != 0, (unsigned)grid, st);
   else launch_extend<f16s>(a, d, interleaved != 0, (unsigned)grid, st);

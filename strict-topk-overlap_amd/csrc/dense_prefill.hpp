@@ -136,33 +136,28 @@ __device__ __forceinline__ int paired(int it, int n, int hkv) {
 // The tile of workgroup wg where every tile has its own.  Neighbouring
 // workgroups take one tile of each KV head, so that with eight heads (or a divisor of
 // eight) an XCD, to which every eighth workgroup goes, reads one head's keys;
-// and within a sequence the last rows, which see the most keys, come first.  Up to 256
+// and within a sequence the last rows, which see the most keys, come first.  Up to 64
 // requests' tiles are laid end to end (four requests of 1024 tokens, one after 16000: 360
 // us, 441 with gaps, which moved long tiles to one CU).  Those of more, which every
 // workgroup would have to add up, come after floor(s G / 128) + r others, s their
 // first row: request r has at least as many places as tiles then (4096 requests of one or
-// two tokens 808 us, 530).
+// two tokens 808 us, 542).
 // kvh = Hkv: none.
 struct TilePlace { int seq, tile, kvh; };
 
 __device__ __forceinline__ TilePlace tile_place(const DenseArgs& a, int wg, int nwg) {
-  __shared__ int s_tmp[4], s_at[2];
   const int it = paired(wg / a.hkv, nwg / a.hkv, a.hkv);
   auto tiles = [&](int rows) { return (int)(((int64_t)rows * a.g + kDenseRows - 1) / kDenseRows); };
   int r = -1, tile = -1;
-  if (a.requests <= 256) {
-    int s0 = 0, s1 = 0, sum;
-    if ((int)threadIdx.x < a.requests) rows_of(a, threadIdx.x, s0, s1);
-    const int c = tiles(s1 - s0);
-    if (threadIdx.x == 0) s_at[0] = -1;
-    const int before = block_excl_scan1(c, s_tmp, &sum);
-    if (it >= before && it < before + c) {
-      s_at[0] = threadIdx.x;
-      s_at[1] = before + c - 1 - it;
+  if (a.requests <= STK_WAVE) {           // (every wave for itself)
+    int s0 = 0, s1 = 0;
+    if (lane_id() < a.requests) rows_of(a, lane_id(), s0, s1);
+    const int c = tiles(s1 - s0), end = wave_incl_scan_dpp(c);
+    const uint64_t mine = __ballot(it >= end - c && it < end);
+    if (mine) {
+      r = __builtin_ctzll(mine);
+      tile = __builtin_amdgcn_readlane(end, r) - 1 - it;
     }
-    __syncthreads();
-    r = s_at[0];
-    tile = s_at[1];
   } else {
     auto before = [&](int i) {
       return (int)((int64_t)min(max(a.starts[i], 0), a.t) * a.g / kDenseRows) + i;
@@ -208,6 +203,21 @@ __device__ __forceinline__ int group_grid(int units, int tk, int launched) {
 
 __device__ __forceinline__ GroupPlace group_place(const DenseArgs& a, int& wg, int launched, int tk,
                                                   int32_t* place) {
+  if (a.ngroups <= STK_WAVE) {            // as in decode_place
+    const int g = lane_id();
+    const int c = g < a.ngroups ? group_tiles(a, g) * group_units(a, g, tk) : 0;
+    const int end = wave_incl_scan_dpp(c);
+    const int per = __builtin_amdgcn_readlane(end, STK_WAVE - 1);
+    if (wg == 0 && (int)threadIdx.x < a.ngroups) place[g] = end - c;
+    if (wg == 0 && threadIdx.x == 0) place[a.ngroups] = per;
+    const Deal deal(per * a.hkv, group_grid(per * a.hkv, tk, launched));
+    if ((uint32_t)wg >= deal.grid) return GroupPlace{0, 0, 0};
+    wg = xcd_remap(wg, (int)deal.grid);
+    const int u = deal.at(wg) % per;
+    const uint64_t mine = __ballot(u >= end - c && u < end);
+    const int at = mine ? __builtin_ctzll(mine) : 0;
+    return GroupPlace{per, at, __builtin_amdgcn_readlane(end - c, at)};
+  }
   __shared__ int s_tmp[4], s_at[2];
   // groups per thread and pass: their loads are in flight together
   const int e = a.ngroups > 256 ? 4 : 1, pass = 256 * e;

@@ -213,6 +213,28 @@ def test_many_requests():
     R.check(got, *R.attention(q, kv, [1] * 700))
 
 
+@pytest.mark.parametrize("requests,groups", [(1500, 1200), (700, 300), (300, 9)])
+def test_many_groups(requests, groups):
+    """Groups of none, one and several requests, more than one pass of the prefix sums takes;
+    requests behind the last group share nothing."""
+    lens = [32 + (i * 7) % 20 for i in range(requests)]
+    kv = R.make(1, 64, 16, lens, BF)
+    at = [(i * (requests - 5) // groups) // 2 * 2 for i in range(groups + 1)]
+    shared = [i % 3 for i in range(groups)]
+    for g, n in enumerate(shared):
+        kv.block_table[at[g]:at[g + 1], :, :n] = kv.block_table[at[g], :, :n]
+    q = R.queries(requests, 2, 64, BF)
+    ints = dict(dtype=torch.int32, device="cuda")
+    got = paged.shared_attention(q, kv, torch.tensor(at, **ints), torch.tensor(shared, **ints))
+    R.check(got, *R.attention(q, kv, [1] * requests))
+
+
+def test_more_requests_than_a_pass():
+    lens = [(i * 37) % 40 for i in range(1300)]
+    kv = R.make(1, 64, 16, lens, FP)
+    _run(R.queries(1300, 2, 64, FP), kv, [1] * 1300)
+
+
 def test_many_rows_without_splitting():
     """Enough row tiles that none is split."""
     kv = R.make(8, 64, 32, [2100] * 2, FP)
@@ -472,6 +494,21 @@ def test_most_listed_requests(requests):
     lens, news = [1 + i % 90 for i in range(requests)], [1] * requests
     kv = R.make(1, 64, 32, lens, FP, width=80)
     _run(R.queries(requests, 1, 64, FP), kv, news, ragged=True)
+
+
+@pytest.mark.parametrize("hq,hkv,d,b", [(136, 1, 64, 1024), (258, 2, 128, 16)])
+def test_more_heads_than_a_tile_has_rows(hq, hkv, d, b):
+    lens = [1500, 3, 0]
+    kv = R.make(hkv, d, b, lens, BF)
+    _run(R.queries(6, hq, d, BF), kv, [3, 3, 0])
+    q = R.queries(3, hq, d, BF)
+    _run(q, kv, [1] * 3)
+    kv.block_table[1, :, :1] = kv.block_table[0, :, :1]
+    ints = dict(dtype=torch.int32, device="cuda")
+    kv.ntokens[1] = b
+    kv.nblocks[1] = 1
+    got = paged.shared_attention(q, kv, torch.tensor([0, 2], **ints), torch.tensor([1], **ints))
+    R.check(got, *R.attention(q, kv, [1] * 3))
 
 
 @pytest.mark.parametrize("mask", ["window", "prefix", "first", "pages"])

@@ -143,6 +143,25 @@ def test_padding_and_many_requests():
     _check(kv, old, q[:t], k[:t], v[:t], news, olds, cos, sin, False, qout[:t])
 
 
+@pytest.mark.parametrize("r,hkv,d,b,most", [(300, 3, 64, 16, 3), (270, 12, 256, 4, 2),
+                                            (300, 2, 128, 64, 12), (5, 20, 128, 8, 2)])
+def test_many_requests_and_heads(r, hkv, d, b, most):
+    """Few tokens of many requests, whose KV heads share workgroups, and more of them."""
+    news = [(i * 7) % (most + 1) for i in range(r)]
+    olds = [(i * 5) % (3 * b) for i in range(r)]
+    kv = R.make(hkv, d, b, [o + m for o, m in zip(olds, news)], BF)
+    kv.ntokens.copy_(torch.tensor(olds, dtype=torch.int32))
+    kv.nblocks.copy_(torch.tensor([-(-o // b) for o in olds], dtype=torch.int32))
+    kv.block_table[r // 2, hkv - 1] = -1
+    old = _copy(kv)
+    t = sum(news)
+    q, k, v = _tokens(t, 2 * hkv, hkv, d, BF)
+    cos, sin = R.tables(kv.width * b, 32)
+    pos = torch.tensor(olds, dtype=torch.int32, device="cuda")
+    qout = paged.extend(kv, k, v, R.starts_of(news), pos, cos, sin, q=q)
+    _check(kv, old, q, k, v, news, olds, cos, sin, False, qout)
+
+
 def test_values_that_are_no_numbers():
     """NaN keys give NaN bounds, as the block bounds do; values pass as bits."""
     kv = R.make(1, 64, 16, [20], BF)

@@ -235,6 +235,36 @@ def test_more_requests_than_a_pass():
     _run(R.queries(1300, 2, 64, FP), kv, [1] * 1300)
 
 
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("dtype,hq,hkv,d,b", [(BF, 16, 8, 64, 32), (FP, 10, 5, 128, 16),
+                                              (BF, 40, 2, 256, 16)])
+def test_many_short_requests(dtype, hq, hkv, d, b, mode):
+    """Short items, several of which lie in one workgroup, of keys all their own and behind
+    shared blocks; what the cache holds behind them is NaN."""
+    lens = [(i * 37) % 300 for i in range(320)]
+    kv = R.make(hkv, d, b, lens, dtype)
+    kw = _kw(hq, mode)
+    q = R.queries(320, hq, d, dtype)
+    ref = R.attention(q, kv, [1] * 320, **kw)
+    table = kv.block_table.tolist()
+    for r, n in enumerate(lens):
+        if n % b:
+            for h in range(hkv):
+                page = table[r][h][n // b]
+                kv.k_pages[page, n % b:] = float("nan")
+                kv.v_pages[page, n % b:] = float("inf")
+    R.check(paged.attention(q, kv, **kw), *ref)
+    ints = dict(dtype=torch.int32, device="cuda")
+    at, shared = list(range(0, 321, 2)), [i % 4 for i in range(160)]
+    for g, n in enumerate(shared):
+        shared[g] = n = min(n, min(lens[2 * g:2 * g + 2]) // b)
+        kv.block_table[2 * g + 1, :, :n] = kv.block_table[2 * g, :, :n]
+    ref = R.attention(q, kv, [1] * 320, **kw)
+    got = paged.shared_attention(q, kv, torch.tensor(at, **ints), torch.tensor(shared, **ints),
+                                 **kw)
+    R.check(got, *ref)
+
+
 def test_many_rows_without_splitting():
     """Enough row tiles that none is split."""
     kv = R.make(8, 64, 32, [2100] * 2, FP)

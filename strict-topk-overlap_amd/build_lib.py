@@ -30,6 +30,7 @@ SOURCES = ["api.cpp", "states.hip", "select.hip", "repair.hip", "signed.hip", "h
            "tail_pg.hip", "stail_pg.hip", "cache.hip", "srepair.hip", "srepair_compact.hip", "compact.hip",
            "hier_mfma.hip", "step1.hip", "repair_fast.hip", "step_small.hip",
            "extend.hip", "dense.hip", "dense_decode_bf16.hip", "dense_decode_f16.hip",
+           "dense_few_bf16.hip", "dense_few_f16.hip",
            "dense_prefill_bf16.hip", "dense_prefill_f16.hip", "dense_direct_bf16.hip",
            "dense_direct_f16.hip", "dense_shared_bf16.hip", "dense_shared_f16.hip"]
 

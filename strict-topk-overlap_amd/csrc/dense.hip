@@ -10,27 +10,31 @@ constexpr int kPlanThreads = 1024;     // and the most requests and tiles that a
 // kWhole (for which there is room to sort them).
 constexpr int kRun = 4, kWhole = 1024;
 
-// Whether `units` units in tiles of at most `most` are better left whole.  A unit
-// takes about 1.4 us on a CU of its own and 2 beside another workgroup (`fill` of
-// them on 256 CUs).  Whole tiles last as long as the longest one, or as all of
-// them dealt out and half the longest one's tail; cut ones are even, but leave
-// parts that k_join_tiles has to read, and each workgroup begins twice: 20 us, and
-// 25 more where every workgroup does.  Causal prompts, 32 query heads over 8 KV
-// heads, D = 128: 1024 tokens (longest tile 16 units) 54 us cut, 37 whole; 2048
-// tokens 95 cut, 65 whole; 471 tokens of 4 heads at D = 256 (33 units, 16
-// tiles) 78 whole.
-__device__ __forceinline__ bool leave_whole(int units, int most, int fill) {
-  const int wgs = min(fill, max(1, units / kRun));
-  const float unit = wgs <= 256 ? 1.4f : 2.f;
-  const float whole = fmaxf(1.4f * most, 2.f * units / fill + 0.7f * most);
-  const float cut = unit * units / wgs + 20.f + 25.f * wgs / 512.f;
+// Whether `units` units in `tiles` tiles of at most `most` are better left whole, in us.
+// A unit takes `one` on a CU of its own, and a CU finishes one per `two` with two
+// workgroups.  Whole tiles last as long as the longest one, or two of them where
+// CUs take two, or as all of them and the longest one's tail; cut ones are even, but leave parts that are written, and read one
+// after the other for a row, and each workgroup begins twice.  The coefficients are fitted to
+// 150 batches of 4 to 760 tiles of 10 to 438 units, measured both ways; the choice is
+// the quicker one or within 8 % of it.  32 query heads over 8 KV
+// heads, D = 128 (whole, cut): 24 tokens after 1400 41.4, 26.9; 500 after 2500 66.3, 52.6;
+// 1500 of three requests after 1400 50.9, 69.1.
+__device__ __forceinline__ bool leave_whole(int units, int most, int tiles, int fill, int d) {
+  const float wgs = (float)min(fill, max(1, units / kRun)), wide = d / 128.f;
+  const float one = d == 64 ? 0.92f : d == 128 ? 1.3f : 1.55f, two = d == 64 ? 0.6f : d == 128 ? 1.f : 1.2f;
+  const float load = tiles <= 256   ? 0.f
+                     : tiles <= 512 ? 1.8f * two * units / tiles
+                                    : two * units / 256.f + 0.2f * most;
+  const float whole = fmaxf(one * most, load);
+  const float cut = (wgs <= 256.f ? one : d == 64 ? 1.3f : 2.2f) * units / wgs + 5.f +
+                    wide * (0.45f * wgs / max(tiles, 1) + 0.02f * wgs + 0.03f * tiles);
   return whole <= cut && most <= kWhole;
 }
 
 // Lists the row tiles: one workgroup.  Within a request the last rows, which see
 // the most keys, come first; whole tiles are listed by their length, the longest
 // first.  fill: workgroups that fill the device.
-__global__ __launch_bounds__(kPlanThreads) void k_plan(DenseArgs a, Plan pl, int tk, int fill) {
+__global__ __launch_bounds__(kPlanThreads) void k_plan(DenseArgs a, Plan pl, int d, int fill) {
   __shared__ int s_a[kPlanThreads / STK_WAVE], s_b[kPlanThreads / STK_WAVE], s_long;
   __shared__ int s_base[kPlanThreads + 1], s_s0[kPlanThreads], s_rows[kPlanThreads],
       s_len[kPlanThreads], s_count[kWhole + 2];
@@ -111,11 +115,12 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan(DenseArgs a, Plan pl, int
   if (lists) {
     if (x.khi <= x.klo) x.klo = x.khi = 0;
     x.kstart = x.klo & ~15;
+    const int tk = d == 256 ? 32 : 64;
     n = max(1, (x.khi - x.kstart + tk - 1) / tk);
     atomicMax(&s_long, n);
   }
   x.cum = block_excl_scan1(n, s_b, &cum);          // (its barrier also publishes s_long)
-  const bool whole = leave_whole(cum * a.hkv, s_long, fill);
+  const bool whole = leave_whole(cum * a.hkv, s_long, rt * a.hkv, fill, d);
   int at = it;
   if (whole) {
     // by length, the longest first; equal ones in any order
@@ -203,12 +208,16 @@ __device__ __forceinline__ void join_parts(const Parts& p, int i0, int count, in
   }
 }
 
-// One row, (request, query head) of a decode batch, per workgroup or, where
+// ALONE: single tokens.  FEW: a few rows per request; rows of no request become zero
+// (a.fill).  SHARED: single tokens, with the parts of their group's shared keys.
+enum JoinKind { ALONE, FEW, SHARED };
+
+// One row, (token, query head) of a decode batch, per workgroup or, where
 // there are enough of them (`WAVE`), per wave: the parts of its own keys, and with
 // SHARED those of its group's shared keys.  Bound by latency (a row's loads are four
 // dependent rounds, about 5 us): 3072 rows of 23 parts took two rounds of
 // workgroups, 13 us, and take 11 as waves; 2560 of 22 at D = 64 11 and 7.6.
-template <typename T, int D, bool SHARED, bool WAVE>
+template <typename T, int D, JoinKind KIND, bool WAVE>
 __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Parts whole,
                                                    const int32_t* place, int launched, Plan pl,
                                                    Parts psplit, Parts pwhole, int plaunched) {
@@ -217,11 +226,24 @@ __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Par
   __shared__ f32x4 s_o[NP][CH];
   const int x = WAVE ? (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(wave_id())
                      : (int)blockIdx.x;
-  if (WAVE && x >= a.requests * a.hq) return;
-  const int r = x / a.hq, head = x % a.hq;
-  const int kvh = head / a.g, gi = head % a.g, nc = decode_chunks(a);
-  const int item = kvh * nc + gi / kDecodeRows, hrow = gi % kDecodeRows;
+  if (WAVE && x >= a.t * a.hq) return;
+  const int tok = x / a.hq, head = x % a.hq, kvh = head / a.g;
   const int tid = WAVE ? lane_id() : (int)threadIdx.x, dc = tid % CH, grp = tid / CH;
+  int r = tok, m0 = 0, rows = 1;                 // the token's place among its request's
+  if constexpr (KIND == FEW) {
+    r = last_at_most(a.requests, tok, [&](int i) { return a.starts[i]; });
+    int s0 = 0, s1 = 0;
+    if (r >= 0) rows_of(a, r, s0, s1);
+    m0 = tok - s0;
+    rows = s1 - s0;
+    if (r < 0 || m0 < 0 || m0 >= rows) {
+      if (a.fill && grp == 0)
+        store_out<T>(a.out + ((int64_t)tok * a.hq + head) * D + 4 * dc, f32x4{}, 0.f);
+      return;
+    }
+  }
+  const int gi = m0 * a.g + head % a.g, nc = row_chunks(a, rows);
+  const int item = kvh * nc + gi / kDecodeRows, hrow = gi % kDecodeRows;
   // a request has the same units for each of its items
   const int base = place[r], end = place[r + 1], total = place[a.requests];
   const int n = (end - base) / (a.hkv * nc), first = base + item * n;
@@ -230,7 +252,7 @@ __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Par
   float m = -INFINITY, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   if (w0 == w1) {
-    if constexpr (!SHARED) return;               // finished by its workgroup
+    if constexpr (KIND != SHARED) return;        // finished by its workgroup
     const int64_t at = ((int64_t)r * a.hkv * nc + item) * kDecodeRows + hrow;
     join_parts(whole, grp, 1, NP, D, 4 * dc, [&](int) { return at; }, m, l, o);
   } else {
@@ -238,7 +260,7 @@ __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Par
       return (2 * (int64_t)(w0 + i) + (i == 0 ? 1 : 0)) * kDecodeRows + hrow;
     }, m, l, o);
   }
-  if constexpr (SHARED) {
+  if constexpr (KIND == SHARED) {
     const int g = group_of(a, r);
     if (g >= 0) {
       int s0, s1;
@@ -290,7 +312,7 @@ __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Par
       }
     }
   }
-  if (grp == 0) store_out<T>(a.out + ((int64_t)r * a.hq + head) * D + 4 * dc, o, l);
+  if (grp == 0) store_out<T>(a.out + ((int64_t)tok * a.hq + head) * D + 4 * dc, o, l);
 }
 
 // ------------------------------------------------------------------ host
@@ -317,17 +339,36 @@ static StkCheck check_dense(const DenseShape& s, int dtype, int pages) {
   return {true, ""};
 }
 
+// Items per KV head of attention in 16 rows, at most.
+static int64_t decode_items(const DenseShape& s) {
+  const int64_t g = s.hq / s.hkv;
+  return s.ragged ? s.tokens * g / kDecodeRows + s.requests
+                  : s.requests * ((g + kDecodeRows - 1) / kDecodeRows);
+}
 static int64_t decode_units(const DenseShape& s) {
-  const int g = s.hq / s.hkv, nc = (g + kDecodeRows - 1) / kDecodeRows;
-  return (int64_t)s.requests * s.hkv * nc * (((int64_t)s.nb * s.b + kUnit - 1) / kUnit + 1);
+  return decode_items(s) * s.hkv * (((int64_t)s.nb * s.b + kUnit - 1) / kUnit + 1);
+}
+// Few rows are worked on as single tokens are, 16 of them at a time: each 16 read
+// the request's keys again, but these are spread over the device, and the reads
+// hit the caches.  So where there are at most as many items as CUs, and their units few, or
+// the rows are about 16 per request (whoever has most of them reads its keys R + 3
+// times at most).  In caches of a few units tiles are as quick.
+// Measured (tiles, items), 32 query heads over 8 KV heads, D = 128: 4 tokens after
+// 2000 42.6, 14.0 us, after 40000 74.6, 38.6; 8 requests of 4 after 2000 44.3, 24.4;
+// 100 tokens after 2000 36.1, 32.9, after 8000 52.3, 107; 32 requests of 4 after 2000
+// 36.6, 41.7.
+constexpr int64_t kFewItems = 256, kFewUnits = 6144;
+static bool few_rows(const DenseShape& s) {
+  return s.ragged && (int64_t)s.nb * s.b > 512 && decode_items(s) * s.hkv <= kFewItems &&
+         (decode_units(s) <= kFewUnits ||
+          (int64_t)s.tokens * (s.hq / s.hkv) <= kDecodeRows * ((int64_t)s.requests + 3));
 }
 // A few items alone are cut into fewer parts (32 each, but one workgroup per CU at
 // least), which the join is quicker with: one request of 16000 tokens, 8 KV
 // heads, D = 128: 23.4 us with 512 workgroups, 21.1 with 256; 32 requests of 200
 // to 2000 tokens: 26.3 and 28.2.
 static int decode_grid(const DenseShape& s) {
-  const int nc = (s.hq / s.hkv + kDecodeRows - 1) / kDecodeRows;
-  const int64_t items = (int64_t)s.requests * s.hkv * nc, u = decode_units(s);
+  const int64_t items = decode_items(s) * s.hkv, u = decode_units(s);
   const int64_t want = items * 32 < kFill / 2 ? kFill / 2 : items * 32;
   const int64_t fill = want < kFill ? want : kFill;
   return (int)(u < fill ? u : fill);
@@ -349,23 +390,21 @@ static int64_t most_units(const DenseShape& s) {
   return (prefill_units(s) / tile_limit(s)) * (rows / kDenseRows + 1) * s.ngroups;
 }
 // Without cutting there is nothing to list and nothing to join, which saves 7 to 12 us.
-// A cache that holds few units leaves little to cut.  Requests of several tiles
-// each fill the device evenly: so do they if there is a tile for every CU and the cache holds
-// a few more units, or tiles enough to fill it several times over.  More than
+// A small cache leaves little to cut, the less the more tiles there are (`holds` times 64
+// keys), and many requests of several tiles each fill the device evenly.  More than
 // k_plan's tiles are not listed.
-// Measured (listed, direct): prompts of 1024 tokens, 32 query heads over 8 KV heads,
-// 36.5, 30 us, of 2048 64, 55.5; 32 requests of 16 tokens after up to 620 29, 22.  With
-// larger caches a tile per CU is not enough: 2900 tokens of 3 requests after up to
-// 12000 418, 574.  128 requests of 4 tokens, one of them after 60000 tokens and the others 500:
-// 153, 1171, and 375, 358 after 4000 each, so short requests are listed.
-constexpr int64_t kDirectUnits = 32, kEvenUnits = 64, kEvenTiles = 4;
+// Measured (listed, direct), 32 query heads over 8 KV heads, D = 128, in full caches:
+// 60 tokens after 600 27.5, 21.5 us, after 1400 30.3, 37.0; 260 after 1400 39.6, 37.7,
+// after 2500 46.3, 57.8; 1000 after 2500 68.4, 61.6; prompts of 2048 tokens 64, 55.5.
+// 128 requests of 4 tokens, one of them after 60000 tokens and the others 500: 153, 1171,
+// and 375, 358 after 4000 each, so short requests are listed.
+constexpr int64_t kSmall = 64, kEvenTiles = 4;
 static bool prefill_direct(const DenseShape& s) {
-  const int tk = s.d == 256 ? 32 : 64;
-  const int64_t tiles = tile_limit(s), holds = (int64_t)s.nb * s.b;
+  const int64_t tiles = tile_limit(s), wgs = tiles * s.hkv;
+  const int64_t holds = ((int64_t)s.nb * s.b + 63) / 64;
   if (s.ngroups) return false;
-  if (tiles > kPlanThreads || holds <= kDirectUnits * tk) return true;
-  return tiles >= kEvenTiles * s.requests &&
-         tiles * s.hkv >= (holds <= kEvenUnits * tk ? kFill / 2 : 2 * kFill);
+  return tiles > kPlanThreads || (holds <= kSmall && wgs >= (s.d == 256 ? 14 : 8) * (holds - 14)) ||
+         (tiles >= kEvenTiles * s.requests && wgs >= 2 * kFill);
 }
 static int prefill_fill(const DenseShape& s) {
   const int64_t u = prefill_units(s);
@@ -407,14 +446,14 @@ static Plan take_plan(Carve& c, const DenseShape& s) {
 }
 
 static size_t dense_bytes(const DenseShape& s) {
-  const int nc = (s.hq / s.hkv + kDecodeRows - 1) / kDecodeRows;
+  const bool few = few_rows(s);
   size_t x = 0;
-  if (!s.ragged) {
+  if (!s.ragged || few) {
     x += stk_align((s.requests + 1) * sizeof(int32_t)) +
          parts_bytes(2 * (int64_t)decode_grid(s), kDecodeRows, s.d);
-    if (s.ngroups) x += parts_bytes((int64_t)s.requests * s.hkv * nc, kDecodeRows, s.d);
+    if (s.ngroups) x += parts_bytes(decode_items(s) * s.hkv, kDecodeRows, s.d);
   }
-  if (s.ragged || s.ngroups) {
+  if ((s.ragged && !few) || s.ngroups) {
     if (!prefill_direct(s))
       x += plan_bytes(s) + parts_bytes(2 * (int64_t)prefill_fill(s), kDenseRows, s.d);
     if (s.ngroups) x += parts_bytes(tile_limit(s) * s.hkv, kDenseRows, s.d);
@@ -423,7 +462,7 @@ static size_t dense_bytes(const DenseShape& s) {
 }
 
 static int launch_plan(const DenseArgs& a, const Plan& p, int d, int fill, hipStream_t st) {
-  hipLaunchKernelGGL(k_plan, dim3(1), dim3(kPlanThreads), 0, st, a, p, d == 256 ? 32 : 64, fill);
+  hipLaunchKernelGGL(k_plan, dim3(1), dim3(kPlanThreads), 0, st, a, p, d, fill);
   return stk_check_launch("k_plan");
 }
 
@@ -438,15 +477,15 @@ static void launch_join_tiles(const DenseArgs& a, const Plan& p, const Parts& sp
 }
 
 constexpr unsigned kJoinAlone = 2048;   // rows that have a workgroup each: one round of them
-template <typename T, bool SHARED>
+template <typename T, JoinKind KIND>
 static void launch_join_rows(const DenseArgs& a, const Parts& split, const Parts& whole,
                              const int32_t* place, int grid, const Plan& p, const Parts& ps,
                              const Parts& pw, int pgrid, int d, hipStream_t st) {
-  const unsigned rows = (unsigned)(a.requests * a.hq);
+  const unsigned rows = (unsigned)(a.t * a.hq);
 #define STK_JOIN(D)                                                                               \
-  (rows <= kJoinAlone ? k_join_rows<T, D, SHARED, false><<<rows, 256, 0, st>>>(                   \
+  (rows <= kJoinAlone ? k_join_rows<T, D, KIND, false><<<rows, 256, 0, st>>>(                   \
                             a, split, whole, place, grid, p, ps, pw, pgrid)                       \
-                      : k_join_rows<T, D, SHARED, true><<<(rows + 3) / 4, 256, 0, st>>>(          \
+                      : k_join_rows<T, D, KIND, true><<<(rows + 3) / 4, 256, 0, st>>>(          \
                             a, split, whole, place, grid, p, ps, pw, pgrid))
   if (d == 64) STK_JOIN(64);
   else if (d == 128) STK_JOIN(128);
@@ -457,7 +496,7 @@ static void launch_join_rows(const DenseArgs& a, const Parts& split, const Parts
 template <typename T>
 static int run_dense(const DenseShape& s, DenseArgs a, int mode, void* workspace, hipStream_t st) {
   Carve c(workspace);
-  if (s.ragged) {
+  if (s.ragged && !few_rows(s)) {
     const int grid = prefill_grid(s);
     if (prefill_direct(s)) return launch_direct<T>(s.d, mode, a, grid, st);
     const Plan p = take_plan(c, s);
@@ -470,24 +509,28 @@ static int run_dense(const DenseShape& s, DenseArgs a, int mode, void* workspace
     launch_join_tiles<T>(a, p, split, s.d, st);
     return stk_check_launch("k_join_tiles");
   }
-  const int nc = (a.g + kDecodeRows - 1) / kDecodeRows;
   const int grid = decode_grid(s);
   int32_t* place = c.take<int32_t>(s.requests + 1);
   const Parts split = take_parts(c, 2 * (int64_t)grid, kDecodeRows, s.d);
   if (s.ngroups) {
-    const Parts whole = take_parts(c, (int64_t)s.requests * s.hkv * nc, kDecodeRows, s.d);
+    const Parts whole = take_parts(c, decode_items(s) * s.hkv, kDecodeRows, s.d);
     const Plan p = take_plan(c, s);
     const int pgrid = prefill_fill(s);
     const Parts ps = take_parts(c, 2 * (int64_t)pgrid, kDenseRows, s.d);
     const Parts pw = take_parts(c, tile_limit(s) * s.hkv, kDenseRows, s.d);
     const int rc = launch_shared<T>(s.d, mode, a, p, ps, pw, pgrid, split, whole, place, grid, st);
     if (rc) return rc;
-    launch_join_rows<T, true>(a, split, whole, place, grid, p, ps, pw, pgrid, s.d, st);
+    launch_join_rows<T, SHARED>(a, split, whole, place, grid, p, ps, pw, pgrid, s.d, st);
   } else {
-    const int rc = launch_decode<T>(s.d, mode, a, split, place, grid, st);
+    const int rc = s.ragged ? launch_few<T>(s.d, mode, a, split, place, grid, st)
+                            : launch_decode<T>(s.d, mode, a, split, place, grid, st);
     if (rc) return rc;
-    launch_join_rows<T, false>(a, split, Parts{}, place, grid, Plan{}, Parts{}, Parts{}, 0, s.d,
+    if (s.ragged)
+      launch_join_rows<T, FEW>(a, split, Parts{}, place, grid, Plan{}, Parts{}, Parts{}, 0, s.d,
                                st);
+    else
+      launch_join_rows<T, ALONE>(a, split, Parts{}, place, grid, Plan{}, Parts{}, Parts{}, 0, s.d,
+                                 st);
   }
   return stk_check_launch("k_join_rows");
 }
@@ -515,7 +558,9 @@ static int dense(const DenseShape& s, const void* q, int64_t q_stride, int dtype
                 reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) &
                15) == 0 && q_stride % 8 == 0 && q_stride >= 0,
               "rows must be 16-byte aligned");
-  STK_REQUIRE(decode_units(s) <= 0x7fffffff && (int64_t)s.requests * s.hq <= 0x7fffffff &&
+  STK_REQUIRE(((s.ragged && !few_rows(s)) || decode_units(s) <= 0x7fffffff) &&
+                  (int64_t)s.requests * s.hq <= 0x7fffffff &&
+                  (int64_t)s.tokens * s.hq <= 0x7fffffff &&
                   most_units(s) <= 0x7fffffff &&
                   (int64_t)s.tokens * (s.hq / s.hkv) + kDenseRows <= 0x7fffffff,
               "batch too large");

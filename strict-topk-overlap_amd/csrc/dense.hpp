@@ -249,10 +249,81 @@ __device__ __forceinline__ Span seq_span(const DenseArgs& a, int q, int s0, int 
   return span_of(a, q, t, p, n);
 }
 
+__device__ __forceinline__ bool nonfinite16(u16x8 v, uint16_t expo) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bad |= (v[i] & expo) == expo;
+  return bad;
+}
+
+// Up to `count` query rows from rown on against the keys [kbase, kend), one row after the
+// other: a lane is a key for the scores and D / 64 dims for the output, and
+// hidden keys and their values are not read.
+template <typename T, int D, int MODE>
+__device__ void slow_rows(const DenseArgs& a, int seq, int s0, int s1, int64_t rown,
+                          int count, int kvh, const int32_t* row, int kbase, int kend,
+                          const Parts* to, int64_t pr) {
+  constexpr int E = D / STK_WAVE;
+  const int lane = lane_id();
+  for (int i = 0; i < count; ++i, ++rown, ++pr) {
+    if (rown >= (int64_t)(s1 - s0) * a.g) return;
+    const int tok = s0 + (int)(rown / a.g), head = kvh * a.g + (int)(rown % a.g);
+    int p;
+    const Span sp = seq_span(a, seq, s0, s1, tok, p);
+    const uint16_t* q = a.q + (int64_t)tok * a.qs + (int64_t)head * D;
+    float slope = 0.f;
+    if constexpr (MODE & 2) slope = a.slopes[head] * 1.44269504f;
+    float m = -INFINITY, l = 0.f, o[E] = {};
+    const int lo = max(kbase, sp.lo), hi = min(kend, sp.hi);
+    for (int k0 = lo & ~15; k0 < hi; k0 += STK_WAVE) {
+      const int key = k0 + lane;
+      const int run = pool_row(a, row, min(key, hi - 1) & ~15);
+      const bool ok = key >= lo && key < hi && run >= 0;
+      const int64_t at = ((int64_t)max(run, 0) + (key & 15)) * D;
+      float s = 0.f;
+      if (ok)
+        for (int x = 0; x < D; ++x) s += cvt(T{q[x]}) * cvt(T{a.kp[at + x]});
+      s = ok ? score2<MODE>(a, s, slope, (float)(p - key)) : -INFINITY;
+      const float mx = fmaxf(m, wave_max(s)), ms = mx == -INFINITY ? 0.f : mx;
+      const float f = part_weight(m, mx), e = ok ? __builtin_amdgcn_exp2f(s - ms) : 0.f;
+      m = mx;
+      l = l * f + wave_sum(e);
+#pragma unroll
+      for (int x = 0; x < E; ++x) o[x] *= f;
+      const uint64_t seen = __ballot(ok);
+      for (int k = 0; k < STK_WAVE; ++k) {
+        if (!(seen >> k & 1)) continue;
+        const float ek = __builtin_bit_cast(
+            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, e), k));
+        const int rk = __builtin_amdgcn_readlane(run, k) + ((k0 + k) & 15);
+#pragma unroll
+        for (int x = 0; x < E; ++x)
+          o[x] += ek * cvt(T{a.vp[(int64_t)rk * D + lane + STK_WAVE * x]});
+      }
+    }
+    if (to) {
+#pragma unroll
+      for (int x = 0; x < E; ++x) to->o[pr * D + lane + STK_WAVE * x] = o[x];
+      if (lane == 0) {
+        to->m[pr] = m;
+        to->l[pr] = l;
+      }
+    } else {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int x = 0; x < E; ++x)
+        a.out[((int64_t)tok * a.hq + head) * D + lane + STK_WAVE * x] = to16<T>(o[x] * inv);
+    }
+  }
+}
+
 // dense_*_{bf16,f16}.hip: one element type each
 template <typename T>
 int launch_decode(int d, int mode, const DenseArgs& a, const Parts& split, int32_t* place, int grid,
                   hipStream_t st);
+template <typename T>
+int launch_few(int d, int mode, const DenseArgs& a, const Parts& split, int32_t* place, int grid,
+               hipStream_t st);
 template <typename T>
 int launch_prefill(int d, int mode, const DenseArgs& a, const Plan& p, const Parts& split, int grid,
                    hipStream_t st);

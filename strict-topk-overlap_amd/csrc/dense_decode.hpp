@@ -1,6 +1,7 @@
-// Dense attention of single tokens over the paged cache.
+// Dense attention of single tokens over the paged cache, and of a few per request (FEW).
 //
-// An item is one request's KV head with up to 16 of its query heads; its keys
+// An item is one request's KV head with up to 16 of its query rows (a token's heads, and
+// with FEW several tokens', each with its own range of keys); its keys
 // are cut into units of kUnit keys, and the units of all items, laid end to end,
 // are dealt evenly over one grid that fills the device: a ragged batch, or one long
 // request, keeps every CU busy to the end.  A workgroup walks its run of units
@@ -27,13 +28,37 @@
 
 namespace stk {
 
-// Decode work of request r: its visible keys, cut into n units from lo16.
-struct DecodeSpan { int lo, hi, lo16, n; };
+// Decode work of request r: the keys that it sees, cut into n units from lo16, and
+// items per KV head.  With starts a request has any number of query tokens, and an
+// item is 16 of their rows (token, head); the keys are those that any of them sees.
+struct DecodeSpan { int lo, hi, lo16, n, nc; };
 
+__device__ __forceinline__ int row_chunks(const DenseArgs& a, int tokens) {
+  return (int)(((int64_t)tokens * a.g + kDecodeRows - 1) / kDecodeRows);
+}
+
+template <bool FEW>
 __device__ __forceinline__ DecodeSpan decode_span(const DenseArgs& a, int r) {
   const int n = tokens_of(a, r);
+  if constexpr (FEW) {
+    int s0, s1;
+    rows_of(a, r, s0, s1);
+    DecodeSpan d{0x7fffffff, 0, 0, 1, row_chunks(a, s1 - s0)};
+    // without documents the spans only move up
+    const int step = a.first ? 1 : max(1, s1 - s0 - 1);
+    for (int t = s0; t < s1; t += step) {
+      const Span s = span_of(a, r, t, n - (s1 - t), n);
+      if (s.hi > s.lo || !a.first) d.lo = min(d.lo, s.lo);
+      if (s.hi > s.lo) d.hi = max(d.hi, s.hi);
+    }
+    if (d.hi <= d.lo) d.lo = d.hi = 0;
+    d.lo16 = d.lo & ~15;
+    if (s1 == s0) d.n = 0;
+    else if (d.hi > d.lo) d.n = (d.hi - d.lo16 + kUnit - 1) / kUnit;
+    return d;
+  }
   const Span s = span_of(a, r, r, n - 1, n);
-  DecodeSpan d{s.lo, s.hi, 0, 1};
+  DecodeSpan d{s.lo, s.hi, 0, 1, row_chunks(a, 1)};
   if (a.groups) {
     const int g = group_of(a, r);
     if (g >= 0) d.lo = max(d.lo, shared_of(a, g));
@@ -43,28 +68,24 @@ __device__ __forceinline__ DecodeSpan decode_span(const DenseArgs& a, int r) {
   return d;
 }
 
-__device__ __forceinline__ int decode_chunks(const DenseArgs& a) {
-  return (a.g + kDecodeRows - 1) / kDecodeRows;
-}
-
 // The requests' units laid end to end: how many there are, the request that holds
 // the first unit of workgroup `wg` of `launched`, and the units before that
 // request (past the last workgroup with work: any).  Workgroup 0 also leaves
 // the units before every request, and their total, in place [R + 1] for k_join_rows.
 struct DecodePlace { int total, base, r; DecodeSpan span; };
 
+template <bool FEW>
 __device__ __forceinline__ DecodePlace decode_place(const DenseArgs& a, int wg, int launched,
                                                     int32_t* place) {
   __shared__ int s_tmp[4], s_at[2];
   __shared__ DecodeSpan s_span;
-  const int per = a.hkv * decode_chunks(a);
   if (a.requests <= STK_WAVE) {
     // every wave looks for itself, without barriers (one request of 16000 tokens 21.3
     // us, 20.5)
     const int r = lane_id();
     DecodeSpan x{};
-    if (r < a.requests) x = decode_span(a, r);
-    const int c = x.n * per, end = wave_incl_scan_dpp(c);
+    if (r < a.requests) x = decode_span<FEW>(a, r);
+    const int c = x.n * x.nc * a.hkv, end = wave_incl_scan_dpp(c);
     const int total = __builtin_amdgcn_readlane(end, STK_WAVE - 1);
     if (wg == 0 && (int)threadIdx.x < a.requests) place[r] = end - c;
     if (wg == 0 && threadIdx.x == 0) place[a.requests] = total;
@@ -76,11 +97,13 @@ __device__ __forceinline__ DecodePlace decode_place(const DenseArgs& a, int wg, 
     p.span.hi = __builtin_amdgcn_readlane(x.hi, at);
     p.span.lo16 = __builtin_amdgcn_readlane(x.lo16, at);
     p.span.n = __builtin_amdgcn_readlane(x.n, at);
+    p.span.nc = __builtin_amdgcn_readlane(x.nc, at);
     return p;
   }
   // requests per thread and pass: their loads are in flight together
   const int e = a.requests > 256 ? 4 : 1, pass = 256 * e;
-  DecodeSpan span[4];
+  DecodeSpan span[4] = {};
+  int units[4];
   // units of this pass's requests before this thread's, and of all of them
   auto scan = [&](int r0, int& before, int& sum) {
     int c = 0;
@@ -88,12 +111,17 @@ __device__ __forceinline__ DecodePlace decode_place(const DenseArgs& a, int wg, 
     for (int j = 0; j < 4; ++j) {
       const int r = r0 + e * (int)threadIdx.x + j;
       span[j].n = 0;
-      if (j < e && r < a.requests) span[j] = decode_span(a, r);
-      c += span[j].n * per;
+      if (j < e && r < a.requests) span[j] = decode_span<FEW>(a, r);
+      units[j] = span[j].n * span[j].nc * a.hkv;
+      c += units[j];
     }
     __syncthreads();
     before = block_excl_scan1(c, s_tmp, &sum);
   };
+  if (threadIdx.x == 0) {
+    s_at[0] = s_at[1] = 0;
+    s_span = DecodeSpan{};
+  }
   int total = 0, before = 0, sum = 0;
   for (int r0 = 0; r0 < a.requests; r0 += pass) {
     scan(r0, before, sum);
@@ -103,7 +131,7 @@ __device__ __forceinline__ DecodePlace decode_place(const DenseArgs& a, int wg, 
       for (int j = 0; j < 4; ++j) {
         const int r = r0 + e * (int)threadIdx.x + j;
         if (j < e && r < a.requests) place[r] = at;
-        at += span[j].n * per;
+        at += units[j];
       }
     }
     total += sum;
@@ -116,7 +144,7 @@ __device__ __forceinline__ DecodePlace decode_place(const DenseArgs& a, int wg, 
     int at = base + before;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int c = span[j].n * per;
+      const int c = units[j];
       if (u >= at && u < at + c) {
         s_at[0] = at;
         s_at[1] = r0 + e * (int)threadIdx.x + j;
@@ -146,9 +174,11 @@ template <int D> constexpr int kDecodeTile = D == 256 ? 16 : 32;
 template <int D> constexpr size_t kDecodeWave = 64 * D;
 template <int D> constexpr size_t kDecodeLds = 4 * kDecodeWave<D>;
 
-// The work of workgroup wg of nwg.  With PARTS items that lie whole in it leave
+// The work of workgroup wg of nwg.  With FEW a value that only some of an item's rows see
+// may be infinite or NaN, and 0 times it is not 0: such an item is done again row by row.
+// With PARTS items that lie whole in it leave
 // their parts in `whole`, too, instead of being finished.
-template <typename T, int D, int MODE, bool PARTS>
+template <typename T, int D, int MODE, bool PARTS, bool FEW = false>
 __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, const Parts& whole,
                                        int32_t* place, char* lds, int wg, int nwg) {
   constexpr int TW = kDecodeTile<D>;    // keys per tile
@@ -158,11 +188,12 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
   constexpr int VN = TW * D / 512;      // 16-byte chunks of a V tile per lane
   constexpr int CPR = D / 8;            // chunks per row
   constexpr int RPI = STK_WAVE / CPR;   // rows per load instruction
+  constexpr uint16_t EXPO = __is_same(T, bf16s) ? 0x7f80 : 0x7c00;
   __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ int s_bad[4];
   const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_id());
   const int n16 = lane & 15, kg = lane >> 4;
-  const int nc = decode_chunks(a);
-  const DecodePlace at = decode_place(a, wg, nwg, place);
+  const DecodePlace at = decode_place<FEW>(a, wg, nwg, place);
   const Deal deal(at.total, nwg);
   if ((uint32_t)wg >= deal.grid) return;
   int u = deal.at(wg);
@@ -190,29 +221,47 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
     sp.hi = __builtin_amdgcn_readfirstlane(sp.hi);
     sp.lo16 = __builtin_amdgcn_readfirstlane(sp.lo16);
     sp.n = __builtin_amdgcn_readfirstlane(sp.n);
-    const int per = a.hkv * nc * sp.n;
+    const int nc = __builtin_amdgcn_readfirstlane(sp.nc), per = a.hkv * nc * sp.n;
     if (u >= base + per) {
+      if (++r >= a.requests) return;      // (starts that decrease may count past the units)
       base += per;
-      next = decode_span(a, ++r);
+      next = decode_span<FEW>(a, r);
       continue;
     }
     const int j0 = (u - base) % sp.n;
-    const bool alone = j0 == 0 && sp.n <= kAlone && u + 4 * sp.n <= min(u1, base + per);
+    // (FEW has too few items for it)
+    const bool alone = !FEW && j0 == 0 && sp.n <= kAlone && u + 4 * sp.n <= min(u1, base + per);
     const int item = (u - base) / sp.n + (alone ? w : 0);
     const int j1 = alone ? sp.n : min(sp.n, j0 + (u1 - u));
     u += alone ? 4 * sp.n : j1 - j0;
-    const int kvh = item / nc, h0 = kvh * a.g + (item % nc) * kDecodeRows;
-    const int gn = min(kDecodeRows, a.g - (item % nc) * kDecodeRows);
+    const int kvh = item / nc, x0 = (item % nc) * kDecodeRows;
+    // rows of the item, and this lane's: token, head, and its range of keys
+    int s0 = r, s1 = r + 1;
+    if constexpr (FEW) rows_of(a, r, s0, s1);
+    const int gn = min(kDecodeRows, (s1 - s0) * a.g - x0), xr = x0 + min(n16, gn - 1);
+    const int tok = FEW ? s0 + xr / a.g : r, head = kvh * a.g + (FEW ? xr % a.g : xr);
+    int p = sp.hi - 1, rlo = sp.lo, rhi = sp.hi, all_lo = sp.lo, all_hi = sp.hi;
+    if constexpr (FEW) {
+      const int n = tokens_of(a, r);
+      p = n - (s1 - tok);
+      const Span rs = span_of(a, r, tok, p, n);
+      const bool some = rs.hi > rs.lo;
+      rlo = some ? rs.lo : 0;
+      rhi = some ? rs.hi : 0;
+      all_lo = (int)wave_ext_u32<true>((uint32_t)rlo);       // keys that every row sees
+      all_hi = (int)wave_ext_u32<false>((uint32_t)rhi);
+    }
+    bool bad = false;
     const int ka = sp.lo16 + j0 * kUnit;
     const int kb = (int)min((int64_t)sp.lo16 + (int64_t)j1 * kUnit, (int64_t)sp.hi);
     const int32_t* row = a.table + ((int64_t)r * a.hkv + kvh) * a.nb;
     // this head's query as the second operand: head n16, dims 32 s + 8 kg ..
     u16x8 qf[KS];
-    const uint16_t* qp = a.q + (int64_t)r * a.qs + (int64_t)(h0 + min(n16, gn - 1)) * D + 8 * kg;
+    const uint16_t* qp = a.q + (int64_t)tok * a.qs + (int64_t)head * D + 8 * kg;
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u16x8*>(qp + 32 * s);
     float slope = 0.f;
-    if constexpr (MODE & 2) slope = a.slopes[h0 + min(n16, gn - 1)] * 1.44269504f;
+    if constexpr (MODE & 2) slope = a.slopes[head] * 1.44269504f;
     float m = -INFINITY, l = 0.f;
     f32x4 acc[DB];
 #pragma unroll
@@ -255,7 +304,7 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
       const int cnt = tb - ta;
       for (int t = 0; t < cnt; ++t) {
         const int key0 = wk + TW * t;
-        bool full = key0 >= sp.lo && key0 + TW <= kb;
+        bool full = key0 >= all_lo && key0 + TW <= min(kb, all_hi);
 #pragma unroll
         for (int y = 0; y < HW; ++y) full = full && rw[y] >= 0;
         if (!full) {
@@ -265,6 +314,7 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
             const int kr = i * RPI + lane / CPR, key = key0 + kr;
             const bool ok = key >= sp.lo && key < kb && rw[i * RPI / 16] >= 0;
             if (!ok) vf[i] = u16x8{};
+            else if (FEW) bad |= nonfinite16(vf[i], EXPO);
           }
         }
         int was[HW];
@@ -281,7 +331,7 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
           for (int y = 0; y < HW; ++y) sq[y] = mma16<T>(kf[y][s], qf[s], sq[y]);
         if (t + 1 < cnt) load(t + 1);
         float x[4 * HW];
-        const float dist = (float)(sp.hi - 1 - key0 - 4 * kg);
+        const float dist = (float)(p - key0 - 4 * kg);
 #pragma unroll
         for (int i = 0; i < 4 * HW; ++i)
           x[i] = score2<MODE>(a, sq[i / 4][i % 4], slope, dist - (float)(16 * (i / 4) + i % 4));
@@ -289,7 +339,7 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
 #pragma unroll
           for (int i = 0; i < 4 * HW; ++i) {
             const int key = key0 + 4 * kg + 16 * (i / 4) + i % 4;
-            x[i] = key >= sp.lo && key < kb && was[i / 4] >= 0 ? x[i] : -INFINITY;
+            x[i] = key >= rlo && key < min(kb, rhi) && was[i / 4] >= 0 ? x[i] : -INFINITY;
           }
         }
         float top = x[0];
@@ -344,14 +394,14 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (alone) {
-      const int64_t pr = ((int64_t)r * a.hkv * nc + item) * kDecodeRows + n16;
+      const int64_t pr = ((int64_t)r * a.hkv * nc + item) * kDecodeRows + n16;   // (PARTS)
       if (n16 < gn) {
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
           if constexpr (PARTS)
             *reinterpret_cast<f32x4*>(whole.o + pr * D + 16 * db + 4 * kg) = acc[db];
           else
-            store_out<T>(a.out + ((int64_t)r * a.hq + h0 + n16) * D + 16 * db + 4 * kg, acc[db], l);
+            store_out<T>(a.out + ((int64_t)tok * a.hq + head) * D + 16 * db + 4 * kg, acc[db], l);
         }
         if (PARTS && kg == 0) {
           whole.m[pr] = m;
@@ -369,12 +419,24 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
       s_m[w][lane] = m;
       s_l[w][lane] = l;
     }
+    if constexpr (FEW) {
+      const bool any = __any(bad);
+      if (lane == 0) s_bad[w] = any;
+    }
     __syncthreads();
     const bool all = j0 == 0 && j1 == sp.n;
     const bool keep = all && !PARTS;                    // finished here
     const Parts& to = all ? whole : split;
     const int64_t slot = all ? (int64_t)r * a.hkv * nc + item
                              : 2 * (int64_t)wg + (j0 > 0 ? 0 : 1);
+    if (FEW && (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3])) {
+      // a value that only some rows see is no number: each row reads its own
+      if (4 * w < gn)
+        slow_rows<T, D, MODE>(a, r, s0, s1, x0 + 4 * w, min(4, gn - 4 * w), kvh, row, ka, kb,
+                              keep ? nullptr : &to, slot * kDecodeRows + 4 * w);
+      __syncthreads();
+      continue;
+    }
     for (int x = threadIdx.x; x < gn * (D / 4); x += 256) {
       const int h = x / (D / 4), dc = x % (D / 4);
       float mx = s_m[0][h];
@@ -391,7 +453,10 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
                      reinterpret_cast<const float*>(lds + i * kDecodeWave<D>) + h * D + 4 * dc);
       }
       if (keep) {
-        store_out<T>(a.out + ((int64_t)r * a.hq + h0 + h) * D + 4 * dc, o, sum);
+        const int y = x0 + h;
+        const int64_t to_row = FEW ? (int64_t)(s0 + y / a.g) * a.hq + kvh * a.g + y % a.g
+                                   : (int64_t)r * a.hq + kvh * a.g + y;
+        store_out<T>(a.out + to_row * D + 4 * dc, o, sum);
       } else {
         const int64_t pr = slot * kDecodeRows + h;
         *reinterpret_cast<f32x4*>(to.o + pr * D + 4 * dc) = o;
@@ -405,11 +470,10 @@ __device__ __forceinline__ void decode(const DenseArgs& a, const Parts& split, c
   }
 }
 
-template <typename T, int D, int MODE>
-__global__ __launch_bounds__(256, 2) void k_decode(DenseArgs a, Parts split,
-                                                                  int32_t* place) {
+template <typename T, int D, int MODE, bool FEW>
+__global__ __launch_bounds__(256, 2) void k_decode(DenseArgs a, Parts split, int32_t* place) {
   __shared__ __attribute__((aligned(16))) char lds[kDecodeLds<D>];
-  decode<T, D, MODE, false>(a, split, split, place, lds, (int)blockIdx.x, (int)gridDim.x);
+  decode<T, D, MODE, false, FEW>(a, split, split, place, lds, (int)blockIdx.x, (int)gridDim.x);
 }
 
 }  // namespace stk

@@ -8,10 +8,10 @@ int launch_decode<f16s>(int d, int mode, const DenseArgs& a, const Parts& split,
                       int grid, hipStream_t st) {
 #define STK_MODE(D)                                                               \
   switch (mode) {                                                                 \
-    case 0: k_decode<f16s, D, 0><<<grid, 256, 0, st>>>(a, split, place); break;   \
-    case 1: k_decode<f16s, D, 1><<<grid, 256, 0, st>>>(a, split, place); break;   \
-    case 2: k_decode<f16s, D, 2><<<grid, 256, 0, st>>>(a, split, place); break;   \
-    default: k_decode<f16s, D, 3><<<grid, 256, 0, st>>>(a, split, place); break;  \
+    case 0: k_decode<f16s, D, 0, false><<<grid, 256, 0, st>>>(a, split, place); break;   \
+    case 1: k_decode<f16s, D, 1, false><<<grid, 256, 0, st>>>(a, split, place); break;   \
+    case 2: k_decode<f16s, D, 2, false><<<grid, 256, 0, st>>>(a, split, place); break;   \
+    default: k_decode<f16s, D, 3, false><<<grid, 256, 0, st>>>(a, split, place); break;  \
   }
   if (d == 64) {
     STK_MODE(64)

@@ -34,13 +34,6 @@
 
 namespace stk {
 
-__device__ __forceinline__ bool nonfinite16(u16x8 v, uint16_t expo) {
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) bad |= (v[i] & expo) == expo;
-  return bad;
-}
-
 // 16 bytes per lane from base + off to LDS, lane after lane from byte `lds`
 // (wave-uniform) on.  Counted by vmcnt like any load; the compiler does not
 // know of the write, so the caller waits (copies_done) and passes a barrier
@@ -63,66 +56,6 @@ __device__ __forceinline__ void copies_done() {
 }
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
-}
-
-// Up to 32 query rows from rown on against the keys [kbase, kend), one row after the
-// other: a lane is a key for the scores and D / 64 dims for the output, and
-// hidden keys and their values are not read.
-template <typename T, int D, int MODE>
-__device__ void slow_rows(const DenseArgs& a, int seq, int s0, int s1, int64_t rown, int kvh,
-                          const int32_t* row, int kbase, int kend, const Parts* to, int64_t pr) {
-  constexpr int E = D / STK_WAVE;
-  const int lane = lane_id();
-  for (int i = 0; i < 32; ++i, ++rown, ++pr) {
-    if (rown >= (int64_t)(s1 - s0) * a.g) return;
-    const int tok = s0 + (int)(rown / a.g), head = kvh * a.g + (int)(rown % a.g);
-    int p;
-    const Span sp = seq_span(a, seq, s0, s1, tok, p);
-    const uint16_t* q = a.q + (int64_t)tok * a.qs + (int64_t)head * D;
-    float slope = 0.f;
-    if constexpr (MODE & 2) slope = a.slopes[head] * 1.44269504f;
-    float m = -INFINITY, l = 0.f, o[E] = {};
-    const int lo = max(kbase, sp.lo), hi = min(kend, sp.hi);
-    for (int k0 = lo & ~15; k0 < hi; k0 += STK_WAVE) {
-      const int key = k0 + lane;
-      const int run = pool_row(a, row, min(key, hi - 1) & ~15);
-      const bool ok = key >= lo && key < hi && run >= 0;
-      const int64_t at = ((int64_t)max(run, 0) + (key & 15)) * D;
-      float s = 0.f;
-      if (ok)
-        for (int x = 0; x < D; ++x) s += cvt(T{q[x]}) * cvt(T{a.kp[at + x]});
-      s = ok ? score2<MODE>(a, s, slope, (float)(p - key)) : -INFINITY;
-      const float mx = fmaxf(m, wave_max(s)), ms = mx == -INFINITY ? 0.f : mx;
-      const float f = part_weight(m, mx), e = ok ? __builtin_amdgcn_exp2f(s - ms) : 0.f;
-      m = mx;
-      l = l * f + wave_sum(e);
-#pragma unroll
-      for (int x = 0; x < E; ++x) o[x] *= f;
-      const uint64_t seen = __ballot(ok);
-      for (int k = 0; k < STK_WAVE; ++k) {
-        if (!(seen >> k & 1)) continue;
-        const float ek = __builtin_bit_cast(
-            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, e), k));
-        const int rk = __builtin_amdgcn_readlane(run, k) + ((k0 + k) & 15);
-#pragma unroll
-        for (int x = 0; x < E; ++x)
-          o[x] += ek * cvt(T{a.vp[(int64_t)rk * D + lane + STK_WAVE * x]});
-      }
-    }
-    if (to) {
-#pragma unroll
-      for (int x = 0; x < E; ++x) to->o[pr * D + lane + STK_WAVE * x] = o[x];
-      if (lane == 0) {
-        to->m[pr] = m;
-        to->l[pr] = l;
-      }
-    } else {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-      for (int x = 0; x < E; ++x)
-        a.out[((int64_t)tok * a.hq + head) * D + lane + STK_WAVE * x] = to16<T>(o[x] * inv);
-    }
-  }
 }
 
 // Workgroups of whole tiles come in the order of their length, and each CU takes
@@ -691,8 +624,8 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
     const int64_t slot = all ? group_slot(a, kvh, seq, s0, tile, pl.limit)
                              : 2 * (int64_t)wg + (j0 > 0 ? 0 : 1);
     if (bad) {
-      slow_rows<T, D, MODE>(a, seq, s0, s0 + nrow, (int64_t)tile * kDenseRows + 32 * w, kvh, row,
-                            kbase, kend, keep ? nullptr : &to, slot * kDenseRows + 32 * w);
+      slow_rows<T, D, MODE>(a, seq, s0, s0 + nrow, (int64_t)tile * kDenseRows + 32 * w, 32, kvh,
+                            row, kbase, kend, keep ? nullptr : &to, slot * kDenseRows + 32 * w);
     }
     l += __shfl_xor(l, 32);
     if (valid && !bad) {

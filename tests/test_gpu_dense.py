@@ -526,6 +526,73 @@ def test_most_listed_requests(requests):
     _run(R.queries(requests, 1, 64, FP), kv, news, ragged=True)
 
 
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("dtype,hq,hkv,d,b", [(BF, 8, 2, 128, 32), (FP, 3, 1, 64, 16),
+                                              (BF, 6, 1, 256, 64), (FP, 20, 2, 256, 16)])
+def test_few_rows(dtype, hq, hkv, d, b, mode):
+    """A few tokens of each request, in 16 rows; rows of no request around them."""
+    lens, news = [2600, 700, 0, 1500, 31, 2], [4, 1, 0, 7, 2, 3]
+    kv = R.make(hkv, d, b, lens, dtype, width=200)
+    t = sum(news)
+    q = R.queries(t + 5, hq, d, dtype)
+    kw = _kw(hq, mode)
+    got = paged.attention(q, kv, R.starts_of(news) + 2, **kw)
+    R.check(got[2:t + 2], *R.attention(q[2:t + 2], kv, news, **kw))
+    assert not bool(got[:2].any()) and not bool(got[t + 2:].any())
+    out = torch.full_like(q, 7.0).contiguous()
+    paged.attention(q, kv, R.starts_of(news) + 2, out=out, **kw)
+    assert torch.equal(out[2:t + 2], got[2:t + 2])
+    assert bool((out[:2] == 7).all()) and bool((out[t + 2:] == 7).all())
+
+
+@pytest.mark.parametrize("mask", ["window", "prefix", "first", "pages", "all"])
+def test_few_rows_masks(mask):
+    lens, news = [2600, 900, 40], [6, 9, 3]
+    kv = R.make(2, 128, 16, lens, FP, width=300)
+    q = R.queries(sum(news), 6, 128, FP)
+    ints = dict(dtype=torch.int32, device="cuda")
+    kw = {}
+    if mask in ("window", "all"):
+        kw["window"] = 700
+    if mask in ("prefix", "all"):
+        kw["prefix"] = torch.tensor([2598, 5000, -3], **ints)
+    if mask in ("first", "all"):
+        first = [p // 37 * 37 for p in range(2594, 2600)] + [890 + i % 3 for i in range(9)] + \
+            [39, 2 ** 31 - 1, -7]
+        kw["first"] = torch.tensor(first, **ints)
+    if mask in ("pages", "all"):
+        kv.block_table[0, 0, 20:130:7] = -1
+        kv.block_table[1, 1, ::2] = kv.pages
+    _run(q, kv, news, **kw)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (FP, 128), (BF, 256)])
+def test_few_rows_hidden_places(dtype, d):
+    """The last token of a request holds no numbers: the ones before it do not see it."""
+    lens, news = [2600, 700, 40], [4, 3, 7]
+    kv = R.make(2, d, 16, lens, dtype, width=200)
+    q = R.queries(sum(news), 6, d, dtype)
+    ref, tol = R.attention(q, kv, news)
+    for r, n in enumerate(lens):
+        for page in kv.block_table[r, :, (n - 1) // 16].tolist():
+            kv.k_pages[page, n % 16:] = float("nan")
+            kv.v_pages[page, n % 16:] = float("nan")
+            kv.v_pages[page, (n - 1) % 16, 5] = float("inf")
+    got = paged.attention(q, kv, R.starts_of(news))
+    last = [3, 6, 13]
+    rest = [i for i in range(14) if i not in last]
+    R.check(got[rest], ref[rest], tol[rest])
+    dims = [i for i in range(d) if i != 5]
+    R.check(got[last][..., dims], ref[last][..., dims], tol[last][..., dims])
+    assert bool(got[last][..., 5].isinf().all())
+
+
+def test_few_rows_of_many_requests():
+    lens, news = [(i * 41) % 500 for i in range(130)], [i % 3 for i in range(130)]
+    kv = R.make(1, 64, 16, lens, BF, width=60)
+    _run(R.queries(sum(news), 2, 64, BF), kv, news)
+
+
 @pytest.mark.parametrize("hq,hkv,d,b", [(136, 1, 64, 1024), (258, 2, 128, 16)])
 def test_more_heads_than_a_tile_has_rows(hq, hkv, d, b):
     lens = [1500, 3, 0]

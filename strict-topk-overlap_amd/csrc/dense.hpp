@@ -121,7 +121,7 @@ __device__ __forceinline__ Span span_of(const DenseArgs& a, int r, int t, int p,
   return span_at(a, r, a.first ? a.first[t] : 0, p, n);
 }
 
-// Shared leading keys of request r (0 outside every group).
+// Shared leading keys of group g.  A request that has fewer reads them itself.
 __device__ __forceinline__ int shared_of(const DenseArgs& a, int g) {
   return (int)min((int64_t)min(max(a.shared[g], 0), a.nb) * a.b, (int64_t)0x7ffffff0);
 }
@@ -241,7 +241,8 @@ __device__ __forceinline__ Span seq_span(const DenseArgs& a, int q, int s0, int 
     const int n = tokens_of(a, t);
     p = n - 1;
     Span s = span_of(a, t, t, p, n);
-    s.hi = min(s.hi, shared_of(a, q));
+    const int keys = shared_of(a, q);
+    s.hi = n < keys ? s.lo : min(s.hi, keys);
     return s;
   }
   const int n = tokens_of(a, q);

@@ -44,12 +44,24 @@ __device__ __forceinline__ DecodeSpan decode_span(const DenseArgs& a, int r) {
     int s0, s1;
     rows_of(a, r, s0, s1);
     DecodeSpan d{0x7fffffff, 0, 0, 1, row_chunks(a, s1 - s0)};
-    // without documents the spans only move up
-    const int step = a.first ? 1 : max(1, s1 - s0 - 1);
-    for (int t = s0; t < s1; t += step) {
-      const Span s = span_of(a, r, t, n - (s1 - t), n);
-      if (s.hi > s.lo || !a.first) d.lo = min(d.lo, s.lo);
-      if (s.hi > s.lo) d.hi = max(d.hi, s.hi);
+    auto see = [&](int t, int first, bool always) {
+      const Span x = span_at(a, r, first, n - (s1 - t), n);
+      if (always || x.hi > x.lo) d.lo = min(d.lo, x.lo);
+      if (x.hi > x.lo) d.hi = max(d.hi, x.hi);
+    };
+    if (a.first && s1 - s0 <= 32) {
+      for (int t = s0; t < s1; t += 8) {
+        int f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = a.first[min(t + i, s1 - 1)];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) see(min(t + i, s1 - 1), f[i], false);
+      }
+    } else if (s1 > s0) {
+      // without documents the spans only move up; documents only raise their lower ends,
+      // and those of more tokens are not looked at
+      see(s0, 0, true);
+      see(s1 - 1, 0, true);
     }
     if (d.hi <= d.lo) d.lo = d.hi = 0;
     d.lo16 = d.lo & ~15;
@@ -61,7 +73,8 @@ __device__ __forceinline__ DecodeSpan decode_span(const DenseArgs& a, int r) {
   DecodeSpan d{s.lo, s.hi, 0, 1, row_chunks(a, 1)};
   if (a.groups) {
     const int g = group_of(a, r);
-    if (g >= 0) d.lo = max(d.lo, shared_of(a, g));
+    const int keys = g >= 0 ? shared_of(a, g) : 0;
+    if (n >= keys) d.lo = max(d.lo, keys);
   }
   d.lo16 = d.lo & ~15;
   if (d.hi > d.lo) d.n = (d.hi - d.lo16 + kUnit - 1) / kUnit;

@@ -120,8 +120,13 @@ __device__ __forceinline__ int group_tiles(const DenseArgs& a, int g) {
   seq_rows(a, g, s0, s1);
   return (int)(((int64_t)(s1 - s0) * a.g + kDenseRows - 1) / kDenseRows);
 }
+// Units of a group's shared keys that its requests' windows hide: they end at or behind
+// the last shared key.
+__device__ __forceinline__ int group_hidden(const DenseArgs& a, int g, int tk) {
+  return a.window > 0 ? max(0, shared_of(a, g) - a.window) / tk : 0;
+}
 __device__ __forceinline__ int group_units(const DenseArgs& a, int g, int tk) {
-  return max(1, (shared_of(a, g) + tk - 1) / tk);
+  return max(1, (shared_of(a, g) + tk - 1) / tk - group_hidden(a, g, tk));
 }
 struct GroupPlace { int per, g, base; };      // per = 0: no work
 
@@ -389,7 +394,7 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
       tl.max_lo = max(max(s_range[0][2], s_range[1][2]), max(s_range[2][2], s_range[3][2]));
       tl.min_hi = min(min(s_range[0][3], s_range[1][3]), min(s_range[2][3], s_range[3][3]));
       if (tl.khi <= tl.klo) tl.klo = tl.khi = 0;
-      if constexpr (KIND == DIRECT) tl.kstart = tl.klo & ~15;
+      tl.kstart = KIND == DIRECT ? tl.klo & ~15 : group_hidden(a, seq, TK) * TK;
     }
     const int kstart = __builtin_amdgcn_readfirstlane(tl.kstart);
     const int klo = __builtin_amdgcn_readfirstlane(tl.klo);
@@ -404,8 +409,8 @@ __device__ __forceinline__ void prefill(const DenseArgs& a, const Plan& pl, cons
     }
     u += whole_tile ? 1 : j1 - j0;
     // units that some row sees (of a group's shared blocks, windows may hide most)
-    const int ja = KIND == GROUPED ? max(j0, klo / TK) : j0;
-    const int jb = KIND == GROUPED ? min(j1, (khi + TK - 1) / TK) : j1;
+    const int ja = KIND == GROUPED ? max(j0, (klo - kstart) / TK) : j0;
+    const int jb = KIND == GROUPED ? min(j1, (khi - kstart + TK - 1) / TK) : j1;
     const int32_t* row = a.table + ((int64_t)(KIND == GROUPED ? s0 : seq) * a.hkv + kvh) * a.nb;
     const int kbase = kstart + ja * TK, kend = min(kstart + jb * TK, khi);
     const int cnt = jb - ja;

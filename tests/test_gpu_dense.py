@@ -388,6 +388,19 @@ def test_shared_groups(groups, shared, kw):
     R.check(paged.shared_attention(q, kv, gs, sh, **kw), *R.attention(q, kv, [1] * 9, **kw))
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("window", [60, 333, 1000, 1300, 2 ** 31 - 1])
+def test_shared_windows(d, window):
+    """Windows that hide most of the shared blocks, in groups of many and of few shared keys, one
+    with requests that hold fewer tokens than are shared."""
+    lens = [1280 + x for x in (0, 1, 40, 300, 1290, 77)] + [1000, 500, 0, 1290, 33, 90]
+    kv = R.make(2, d, 16, lens, BF)
+    gs, sh = _share(kv, [0, 6, 10, 12], [80, 70, 2])
+    q = R.queries(12, 40, d, BF)
+    R.check(paged.shared_attention(q, kv, gs, sh, window=window),
+            *R.attention(q, kv, [1] * 12, window=window))
+
+
 def test_shared_long_prefix_many_rows():
     """More query rows than one tile and keys enough to be split."""
     lens = [2048 + 1 + 3 * i for i in range(45)]
@@ -585,6 +598,17 @@ def test_few_rows_hidden_places(dtype, d):
     dims = [i for i in range(d) if i != 5]
     R.check(got[last][..., dims], ref[last][..., dims], tol[last][..., dims])
     assert bool(got[last][..., 5].isinf().all())
+
+
+@pytest.mark.parametrize("mode", MODES)
+def test_few_rows_of_many_documents(mode):
+    """More tokens of a request than its documents are looked at, and fewer."""
+    lens, news = [900, 650], [90, 30]
+    kv = R.make(1, 64, 16, lens, BF, width=60)
+    q = R.queries(sum(news), 2, 64, BF)
+    pos = [n - m + t for n, m in zip(lens, news) for t in range(m)]
+    first = torch.tensor([p // 23 * 23 for p in pos], dtype=torch.int32, device="cuda")
+    _run(q, kv, news, first=first, **_kw(2, mode))
 
 
 def test_few_rows_of_many_requests():

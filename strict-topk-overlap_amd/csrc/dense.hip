@@ -215,7 +215,7 @@ enum JoinKind { ALONE, FEW, SHARED };
 // One row, (token, query head) of a decode batch, per workgroup or, where
 // there are enough of them (`WAVE`), per wave: the parts of its own keys, and with
 // SHARED those of its group's shared keys.  Bound by latency (a row's loads are four
-// dependent rounds, about 5 us): 3072 rows of 23 parts took two rounds of
+// dependent rounds, about 5 us): 96 requests of 32 heads and 23 parts took two rounds of
 // workgroups, 13 us, and take 11 as waves; 2560 of 22 at D = 64 11 and 7.6.
 template <typename T, int D, JoinKind KIND, bool WAVE>
 __global__ __launch_bounds__(256) void k_join_rows(DenseArgs a, Parts split, Parts whole,

@@ -4,7 +4,7 @@
 // blocks, each tile 128 query rows of a group's requests (dense_prefill.hpp), the others
 // on the requests' own keys (dense_decode.hpp).  All leave parts, which
 // k_join_rows joins.  96 requests, 32 query heads over 8, D = 128, of which 32768 keys
-// are shared and 1 to 2000 their own: 95 us, 62 of them on the shared blocks' 51
+// are shared and 1 to 2000 their own: 90 us, 62 of them on the shared blocks' 51
 // GFLOP, then 20 to 30 on the others' 100 MB (a CU holds two workgroups of
 // either kind, so the kinds hardly overlap), and 11 for the join of 33 MB of parts.
 #pragma once

@@ -336,6 +336,25 @@ def test_captured_graph_follows_lengths():
         R.check(many, *R.attention(qr, kv, [s1, 60 - s1]))
 
 
+def test_captured_graph_of_listed_tiles():
+    """Tiles that the device lists, cut and leaves whole from one replay to the next."""
+    kv = R.make(2, 128, 16, [3000, 600], BF, width=200)
+    q = R.queries(600, 8, 128, BF)
+    starts = R.starts_of([40, 560])
+    paged.attention(q, kv, starts)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = paged.attention(q, kv, starts)
+    for n0, n1, s1 in ((3000, 600, 40), (300, 300, 300), (3000, 40, 590), (2, 580, 20), (0, 0, 0)):
+        kv.ntokens.copy_(torch.tensor([n0, n1], dtype=torch.int32))
+        starts.copy_(torch.tensor([0, s1, 600], dtype=torch.int32))
+        q.copy_(R.queries(600, 8, 128, BF, seed=n0 + 1))
+        g.replay()
+        torch.cuda.synchronize()
+        R.check(got, *R.attention(q, kv, [s1, 600 - s1]))
+        R.check(paged.attention(q, kv, starts), *R.attention(q, kv, [s1, 600 - s1]))
+
+
 def test_concurrent_streams():
     kv = R.make(2, 64, 16, [500, 41], FP)
     q = R.queries(2, 4, 64, FP)

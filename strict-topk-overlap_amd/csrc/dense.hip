@@ -10,18 +10,19 @@ constexpr int kPlanThreads = 1024;     // and the most requests and tiles that a
 // kWhole (for which there is room to sort them).
 constexpr int kRun = 4, kWhole = 1024;
 
-// Whether `units` units in `tiles` tiles of at most `most` are better left whole, in us.
-// A unit takes `one` on a CU of its own, and a CU finishes one per `two` with two
-// workgroups.  Whole tiles last as long as the longest one, or two of them where
-// CUs take two, or as all of them and the longest one's tail; cut ones are even, but leave parts that are written, and read one
-// after the other for a row, and each workgroup begins twice.  The coefficients are fitted to
-// 150 batches of 4 to 760 tiles of 10 to 438 units, measured both ways; the choice is
-// the quicker one or within 8 % of it.  32 query heads over 8 KV
-// heads, D = 128 (whole, cut): 24 tokens after 1400 41.4, 26.9; 500 after 2500 66.3, 52.6;
-// 1500 of three requests after 1400 50.9, 69.1.
+// Whether `units` units in `tiles` tiles of at most `most` are better left whole; times
+// in us.  A unit takes `one` on a CU of its own, and a CU finishes one per `two` with
+// two workgroups.  Whole tiles last as long as the longest one, or two of them where
+// CUs take two, or as all of them and the longest one's tail; cut ones are even, but
+// leave parts that are written, and read one after the other for a row, and each
+// workgroup begins twice.  The coefficients are fitted to 216 batches of 4 to 760 tiles of
+// 10 to 438 units, measured both ways: the choice is the quicker one or within 7 % of
+// it.  32 query heads over 8 KV heads, D = 128 (whole, cut): 24 tokens after 1400 41.4,
+// 26.9; 500 after 2500 66.3, 52.6; 1500 of three requests after 1400 50.9, 69.1.
 __device__ __forceinline__ bool leave_whole(int units, int most, int tiles, int fill, int d) {
   const float wgs = (float)min(fill, max(1, units / kRun)), wide = d / 128.f;
-  const float one = d == 64 ? 0.92f : d == 128 ? 1.3f : 1.55f, two = d == 64 ? 0.6f : d == 128 ? 1.f : 1.2f;
+  const float one = d == 64 ? 0.92f : d == 128 ? 1.3f : 1.55f;
+  const float two = d == 64 ? 0.6f : d == 128 ? 1.f : 1.2f;
   const float load = tiles <= 256   ? 0.f
                      : tiles <= 512 ? 1.8f * two * units / tiles
                                     : two * units / 256.f + 0.2f * most;
@@ -551,7 +552,8 @@ static int dense(const DenseShape& s, const void* q, int64_t q_stride, int dtype
   STK_REQUIRE(s.tokens == 0 || (q && out), "null pointer");
   STK_REQUIRE(k_pages && v_pages && table && nblocks, "null pointer");
   STK_REQUIRE(scale > 0.f && scale <= kMaxScale, "scale must be positive and at most 1e30");
-  STK_REQUIRE(softcap >= 0.f && softcap <= kMaxCap && (softcap == 0.f || scale / softcap <= kMaxScale),
+  STK_REQUIRE(softcap >= 0.f && softcap <= kMaxCap &&
+                  (softcap == 0.f || scale / softcap <= kMaxScale),
               "softcap must be in (0, 4096], 0 for none, and not far below the scale");
   STK_REQUIRE(window >= 0, "window must be at least 0 (0: none)");
   STK_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) |

@@ -214,7 +214,7 @@ struct Deal {
 // [max_lo, min_hi).
 struct Tile { int seq, tile, kstart, cum, klo, khi, max_lo, min_hi, s0, rows, len; };
 struct Plan {
-  int32_t* head;      // {units per KV head, tiles, workgroups that the units are dealt to (0: tiles are whole)}
+  int32_t* head;      // {units per KV head, tiles, workgroups of the units (0: whole tiles)}
   Tile* tiles;
   int32_t* base;      // with groups, instead of a list: [groups + 1] units before each
   int limit;          // most tiles there can be

@@ -10,7 +10,8 @@
 // the host.
 //
 // Within a workgroup the four waves take a quarter of the keys each (short items:
-// one item each) and share nothing until the item ends.  A wave's tile is 32 keys (at D = 256 it is 16):
+// one item each) and share nothing until the item ends.  A wave's tile is 32 keys
+// (at D = 256 it is 16):
 //   S[key, head] = K Q^T  (16x16x32, K straight from global memory to registers,
 //                          in the operand's own layout),
 //   O^T[dim, head] += V^T P^T  (V through the wave's own LDS, read transposed).

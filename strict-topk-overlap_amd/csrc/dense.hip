@@ -360,7 +360,9 @@ static int64_t decode_units(const DenseShape& s) {
 // 36.6, 41.7.
 constexpr int64_t kFewItems = 256, kFewUnits = 6144;
 static bool few_rows(const DenseShape& s) {
+  // (the units fit an int even if starts that decrease give every request all rows)
   return s.ragged && (int64_t)s.nb * s.b > 512 && decode_items(s) * s.hkv <= kFewItems &&
+         s.requests * decode_units(s) <= 0x7fffffff &&
          (decode_units(s) <= kFewUnits ||
           (int64_t)s.tokens * (s.hq / s.hkv) <= kDecodeRows * ((int64_t)s.requests + 3));
 }
